@@ -138,6 +138,35 @@ int llkv_rope_append(void* q, void* k, const void* v, void* k_pool, void* v_pool
                      int num_tokens, int num_q_heads, int num_kv_heads, int head_dim,
                      int rotary_dim, int dtype, void* stream);
 
+/* Per-head RMS norm of queries and keys, rotation by one or several position
+ * axes and KV append in one pass.  Additive: the reference has neither the norm
+ * nor several axes; llkv_rope_append is the form with tables built by the
+ * caller.  Per head row x of D elements of token t:
+ *     y   = x * w / sqrt(mean(x^2) + eps)            (w null: y = x)
+ *     phi = positions[axis(i)][t] * inv_freq[i],  i < rotary_dim / 2
+ *     out = (y1 cos phi - y2 sin phi, y2 cos phi + y1 sin phi)
+ * for the pairs (i, i + rotary_dim / 2); dims >= rotary_dim take y.  fp32
+ * arithmetic, angles reduced in fp64, one rounding to the element type.
+ * q [num_tokens, Hq, D], k and v [num_tokens, Hkv, D]: each token's heads are
+ * contiguous and tokens are *_stride elements apart (slices of one fused
+ * projection).  q (may be NULL) goes to q_out; k and v rows go to pool row
+ * slot_mapping[t] (negative: no pool write) and, with k_out not NULL, the k row
+ * to k_out as well.  q_out / k_out may be q / k themselves (same stride);
+ * otherwise inputs and outputs must not overlap.
+ * positions: device int32 [num_axes, num_tokens]; 1 <= num_axes <= 4.
+ * pair_axis: HOST array of rotary_dim / 2 axis numbers (NULL with one axis).
+ * inv_freq: device fp32 [rotary_dim / 2].  q_weight, k_weight: device fp32 [D]
+ * or NULL (no norm).  rotary_dim even, 0 <= rotary_dim <= D <= 256 (0: no
+ * rotation, positions and inv_freq may be NULL). */
+int llkv_qk_norm_rope_append(void* q_out, void* k_out, const void* q, const void* k, const void* v,
+                             int64_t q_out_stride, int64_t k_out_stride, int64_t q_stride,
+                             int64_t k_stride, int64_t v_stride, void* k_pool, void* v_pool,
+                             const int64_t* slot_mapping, const int* positions, int num_axes,
+                             const uint8_t* pair_axis, const float* inv_freq,
+                             const float* q_weight, const float* k_weight, float eps,
+                             int num_tokens, int num_q_heads, int num_kv_heads, int head_dim,
+                             int rotary_dim, int dtype, void* stream);
+
 /* ------------------------------------------------------------------------
  * Paged decode attention (one new token per sequence), with Split-K.
  * Replaces lightllm::kv_cache::paged_attention
@@ -275,6 +304,110 @@ int llkv_paged_prefill(void* out, const void* q, const void* k_pool,
                        int num_kv_heads, int head_dim, int block_size,
                        int causal, float scale, int dtype, void* workspace,
                        size_t workspace_bytes, void* stream);
+
+/* ------------------------------------------------------------------------
+ * Drafted trees (additive: the reference drafts single chains).
+ * A sequence's last P = cu_q[n+1] - cu_q[n] keys are the nodes of a tree that a
+ * draft proposed, appended in any order in which parents come first; node i is
+ * row cu_q[n] + i of q and sits at cache position seq_lens[n] - P + i.
+ * ------------------------------------------------------------------------ */
+
+/* Ancestor masks and positions from parent indices.  parents: device int32
+ * [total_q], node i's parent within its sequence; a value outside [0, i) makes
+ * node i a root.  Row i of tree_mask (device int32 [total_q, mask_words],
+ * mask_words >= ceil(max_q_len / 32)) gets bit j (word j / 32, bit j % 32) for
+ * node i itself and each of its ancestors.  positions (may be NULL): device
+ * int32 [total_q], the context's length plus the node's depth, for the rotation. */
+int llkv_build_tree(int* tree_mask, int mask_words, int* positions, const int* parents,
+                    const int* cu_q, const int* seq_lens, int num_seqs, int total_q,
+                    int max_q_len, void* stream);
+
+/* Attention of a tree's nodes over the paged cache: node i sees every key of
+ * the context (positions below seq_lens[n] - P) and those nodes j of its own
+ * sequence whose bit is set in row cu_q[n] + i of tree_mask (any mask, not
+ * only an ancestor mask; bits >= P are ignored).  A row that sees no key gives
+ * zeros.  K and V of keys that a row does not see have no effect on it, whatever
+ * they hold.  Other arguments as llkv_paged_prefill; max_q_len and max_seq_len
+ * only size the launch, results follow cu_q and seq_lens.
+ * workspace: llkv_paged_tree_attention_workspace_size() bytes, 16-byte aligned,
+ * uninitialised; calls that share it must not overlap. */
+size_t llkv_paged_tree_attention_workspace_size(int num_seqs, int max_q_len, int num_q_heads,
+                                                int num_kv_heads, int head_dim, int block_size,
+                                                int max_seq_len, int dtype);
+int llkv_paged_tree_attention(void* out, const void* q, const void* k_pool,
+                              const void* v_pool, const int* block_table,
+                              int max_blocks_per_seq, const int* cu_q, const int* seq_lens,
+                              const int* tree_mask, int mask_words, int num_seqs, int total_q,
+                              int max_q_len, int max_seq_len, int num_q_heads,
+                              int num_kv_heads, int head_dim, int block_size, float scale,
+                              int dtype, void* workspace, size_t workspace_bytes,
+                              void* stream);
+
+/* ------------------------------------------------------------------------
+ * Accumulated attention weights and eviction (additive).
+ * mass: device fp32, the total of key j of kv head h of sequence n at
+ * mass[n * mass_seq_stride + h * mass_head_stride + j]: the sum, over the
+ * queries so far and the query heads of h, of the softmax weight of key j.
+ * Rows hold at least max_seq_len totals, which the caller starts at zero; those
+ * of positions >= seq_lens[n] are left as they are.  Each sequence has rows of
+ * its own (rows that two sequences share would race).  Keys beyond max_seq_len
+ * are cut off here: the bound must hold.
+ * ------------------------------------------------------------------------ */
+
+/* llkv_paged_decode that adds the step's weights to the totals as well, reading
+ * K and V once.  At most 64 query heads per kv head.  workspace as above. */
+size_t llkv_paged_decode_mass_workspace_size(int num_seqs, int num_q_heads, int num_kv_heads,
+                                             int head_dim, int block_size, int max_seq_len,
+                                             int dtype);
+int llkv_paged_decode_mass(void* out, float* mass, int64_t mass_seq_stride,
+                           int64_t mass_head_stride, const void* q, const void* k_pool,
+                           const void* v_pool, const int* block_table, const int* seq_lens,
+                           int num_seqs, int num_q_heads, int num_kv_heads, int head_dim,
+                           int block_size, int max_blocks_per_seq, int max_seq_len,
+                           float scale, int dtype, void* workspace, size_t workspace_bytes,
+                           void* stream);
+
+/* Adds the weights that the given rows give to each key, without an attention
+ * output: the last P = cu_q[n+1] - cu_q[n] tokens of sequence n, whose queries
+ * are rows cu_q[n] .. of q and which see the keys up to their own positions (as
+ * llkv_paged_prefill with causal set), for instance the last 32 of a prompt. */
+size_t llkv_paged_window_mass_workspace_size(int total_q, int num_q_heads, int max_seq_len,
+                                             int dtype);
+int llkv_paged_window_mass(float* mass, int64_t mass_seq_stride, int64_t mass_head_stride,
+                           const void* q, const void* k_pool, const int* block_table,
+                           int max_blocks_per_seq, const int* cu_q, const int* seq_lens,
+                           int num_seqs, int total_q, int max_q_len, int max_seq_len,
+                           int num_q_heads, int num_kv_heads, int head_dim, int block_size,
+                           float scale, int dtype, void* workspace, size_t workspace_bytes,
+                           void* stream);
+
+/* The keys to keep, per (sequence, kv head): counts[n] = min(seq_lens[n],
+ * budget) positions in rising order in keep [num_seqs, Hkv, budget] (device
+ * int32, -1 behind the last): all of them when they fit; otherwise the first
+ * `sinks`, the last `recent` (sinks + recent <= budget), and of the others those
+ * with the largest totals, ties going to the lower position; a NaN total is
+ * below every number.  mass_out (rows of out_width >= min(budget, max_seq_len)
+ * values; not overlapping mass) gets the kept totals in the same order, then
+ * zeros.  seq_lens beyond max_seq_len are cut off at it. */
+int llkv_evict_select(int* keep, int* counts, float* mass_out, int64_t out_seq_stride,
+                      int64_t out_head_stride, int out_width, const float* mass,
+                      int64_t mass_seq_stride, int64_t mass_head_stride, const int* seq_lens,
+                      int num_seqs, int num_kv_heads, int max_seq_len, int budget, int sinks,
+                      int recent, void* stream);
+
+/* Moves rows of K and V, bit for bit: position keep[n][h][i] of sequence n (of
+ * kv head h; keep_heads 1: of all heads) to position dst_start[n] + i
+ * (dst_start NULL: i), for i < counts[n].  keep: device int32 [num_seqs,
+ * keep_heads, max_keep]; counts, dst_start: device int32 [num_seqs].
+ * dst_table not NULL: to the pages of dst_table, none of which the call reads.
+ * dst_table NULL: within src_table's pages; keep must then rise and have
+ * keep[i] >= dst_start + i, and the pages moved must be the sequence's own (not
+ * a prefix that others share).  Positions outside a table, or on a -1 entry, are
+ * neither read nor written. */
+int llkv_compact(void* k_pool, void* v_pool, const int* src_table, int src_max_blocks,
+                 const int* dst_table, int dst_max_blocks, const int* keep, int keep_heads,
+                 int max_keep, const int* counts, const int* dst_start, int num_seqs,
+                 int num_kv_heads, int head_dim, int block_size, int dtype, void* stream);
 
 /* Replaces first_prefill_attn_batched_gpu[_dispatch]
  * (include/lightllm/kv_cache/paged_attention.h:130-145,

@@ -43,6 +43,22 @@ _SIGS = {
     "llkv_build_slots": (c_int, [c_void_p, c_void_p, c_int, c_void_p, c_void_p, c_int, c_int, c_int,
                                  c_void_p]),
     "llkv_rope_append": (c_int, [c_void_p] * 8 + [c_int] * 6 + [c_void_p]),
+    "llkv_qk_norm_rope_append": (c_int, [c_void_p] * 5 + [c_int64] * 5 + [c_void_p] * 4
+                                 + [c_int, c_char_p] + [c_void_p] * 3 + [c_float] + [c_int] * 6 + [c_void_p]),
+    "llkv_build_tree": (c_int, [c_void_p, c_int] + [c_void_p] * 4 + [c_int] * 3 + [c_void_p]),
+    "llkv_paged_tree_attention_workspace_size": (c_size_t, [c_int] * 8),
+    "llkv_paged_tree_attention": (c_int, [c_void_p] * 5 + [c_int] + [c_void_p] * 3 + [c_int] * 9
+                                  + [c_float, c_int, c_void_p, c_size_t, c_void_p]),
+    "llkv_paged_decode_mass_workspace_size": (c_size_t, [c_int] * 7),
+    "llkv_paged_decode_mass": (c_int, [c_void_p, c_void_p, c_int64, c_int64] + [c_void_p] * 5 + [c_int] * 7
+                               + [c_float, c_int, c_void_p, c_size_t, c_void_p]),
+    "llkv_paged_window_mass_workspace_size": (c_size_t, [c_int] * 4),
+    "llkv_paged_window_mass": (c_int, [c_void_p, c_int64, c_int64] + [c_void_p] * 3 + [c_int] + [c_void_p] * 2
+                               + [c_int] * 8 + [c_float, c_int, c_void_p, c_size_t, c_void_p]),
+    "llkv_evict_select": (c_int, [c_void_p] * 3 + [c_int64, c_int64, c_int, c_void_p, c_int64, c_int64, c_void_p]
+                          + [c_int] * 6 + [c_void_p]),
+    "llkv_compact": (c_int, [c_void_p] * 3 + [c_int, c_void_p, c_int, c_void_p, c_int, c_int, c_void_p, c_void_p]
+                     + [c_int] * 5 + [c_void_p]),
     "llkv_paged_decode_workspace_size": (c_size_t, [c_int, c_int, c_int, c_int, c_int, c_int, c_int]),
     "llkv_paged_decode": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int,
                                   c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_float, c_int,

@@ -1,0 +1,360 @@
+// The attention weight that the last rows of each sequence give to each of its
+// keys, summed over rows and query heads and added to the keys' totals (gfx950).
+//
+// For a sequence of L keys whose last P rows are given, row i (at position
+// L - P + i) seeing keys j <= L - P + i:
+//     total[h][j] += sum over rows i and the heads c of kv head h of
+//                    exp(x_ijc - lse_ic),   x = scale q_ic . k_j.
+// The scores (4 bytes for each of the P G columns of a key) are more than the
+// key's K row, so they are computed twice rather than stored: once for each
+// column's log-sum-exp, once for the sums.  Both passes hold a block of keys in
+// the operand registers of the matrix instructions (K as in the decode) and run
+// over the columns, so that K is read once a pass, a key's sum stays in one
+// wave's registers and nothing is added atomically.
+#include <hip/hip_runtime.h>
+
+#include <algorithm>
+
+#include "attn_common.h"
+#include "decode_mfma.h"
+
+namespace llkv {
+namespace {
+
+constexpr int kWaves = 4;
+
+struct WindowArgs {
+    const void* q;
+    const void* k;
+    const int* bt;
+    const int* cu_q;
+    const int* lens;
+    int max_blocks, N, Hq, Hkv, D, bs, max_len;
+    float scale_log2;
+    int nblk;          // key blocks of a sequence (by the bound)
+    float* part;       // [rows * Hq][nblk] log2-sum-exp2 per key block
+    float* lse;        // [rows * Hq]
+    float* mass;
+    int64_t mass_bs, mass_hs;
+};
+
+struct WindowSeq {
+    int q0, P, L, hist;
+};
+
+__device__ inline WindowSeq window_seq(const WindowArgs& a, int n) {
+    WindowSeq s;
+    s.q0 = a.cu_q[n];
+    s.P = max(a.cu_q[n + 1] - s.q0, 0);
+    const int l = a.lens[n], cap = min(a.max_blocks * a.bs, a.max_len);
+    s.L = l < 0 ? 0 : (l > cap ? cap : l);
+    s.hist = s.L - s.P;
+    return s;
+}
+
+// Keys per wave: as many 16-key tiles as leave registers for two waves per SIMD.
+template <typename T>
+constexpr int key_tiles() { return Elem<T>::kDtype == LLKV_DTYPE_F32 ? 2 : 4; }
+template <typename T>
+constexpr int block_keys() { return kWaves * 16 * key_tiles<T>(); }
+
+// SUM false: part[column][block] = the block's log2-sum-exp2 of each column.
+// SUM true: the totals, from the columns' log2-sum-exp2.
+// Grid (nblk, Hkv, N).
+template <typename T, int D, bool SUM>
+__global__ __launch_bounds__(256) void window_kernel(WindowArgs a) {
+    using Ops = ScoreOps<T, D>;
+    constexpr int KT = key_tiles<T>();
+    __shared__ float ml[2][kWaves][16][2];   // SUM false: the waves' (max, sum) of a column tile
+    const int n = blockIdx.z, kvh = blockIdx.y;
+    const WindowSeq s = window_seq(a, n);
+    const int k0 = blockIdx.x * block_keys<T>();
+    if (k0 >= s.L || s.P == 0) return;
+    const int lane = threadIdx.x & 63, g = lane >> 4, c = lane & 15;
+    const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int G = a.Hq / a.Hkv, cols = s.P * G;
+    const int64_t row_elems = (int64_t)a.Hkv * D;
+    const int* bt = a.bt + (int64_t)n * a.max_blocks;
+    const int npages = (s.L + kPage - 1) / kPage;
+
+    typename Ops::KReg kr[KT][Ops::NK];
+    int p0[KT];   // the tile's first position
+#pragma unroll
+    for (int kt = 0; kt < KT; ++kt) {
+        p0[kt] = k0 + (w * KT + kt) * kPage;
+        const int64_t phys = max(bt[min(p0[kt] / kPage, npages - 1)], 0);   // (beyond the last page: masked)
+        Ops::template load_k<false>(reinterpret_cast<const T*>(a.k) + (int64_t)kvh * D + (phys * kPage + c) * row_elems,
+                                    g, kr[kt]);
+    }
+    const bool whole = p0[KT - 1] + kPage <= s.hist;   // every row sees all of the wave's keys (uniform)
+
+    float sum[KT][4];
+#pragma unroll
+    for (int kt = 0; kt < KT; ++kt)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) sum[kt][i] = 0.0f;
+
+    for (int c0 = 0; c0 < cols; c0 += 16) {
+        const int col = c0 + c;
+        const bool valid = col < cols;
+        const int node = valid ? col / G : 0;
+        const int64_t qrow = (int64_t)(s.q0 + node) * a.Hq + kvh * G + (col - node * G);
+        typename Ops::QReg q[Ops::NQ];
+        Ops::load_q(reinterpret_cast<const T*>(a.q) + qrow * D, valid, g, a.scale_log2, q);
+        const int last = valid ? min(s.hist + node, s.L - 1) : -1;   // the last key that the column sees
+        const float lse = SUM && valid ? a.lse[qrow] : INFINITY;
+        mf32x4 x[KT];
+#pragma unroll
+        for (int kt = 0; kt < KT; ++kt) {
+            x[kt] = Ops::scores(kr[kt], q, a.scale_log2);
+            if (!whole) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    if (p0[kt] + 4 * g + i > last) x[kt][i] = -INFINITY;
+            }
+        }
+        if constexpr (SUM) {
+#pragma unroll
+            for (int kt = 0; kt < KT; ++kt)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) sum[kt][i] += fast_exp2(x[kt][i] - lse);
+        } else {
+            float m = -INFINITY;
+#pragma unroll
+            for (int kt = 0; kt < KT; ++kt)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) m = fmaxf(m, x[kt][i]);
+            m = fmaxf(m, __shfl_xor(m, 16, 64));
+            m = fmaxf(m, __shfl_xor(m, 32, 64));
+            m = fmaxf(m, kNegBig);
+            float l = 0.0f;
+#pragma unroll
+            for (int kt = 0; kt < KT; ++kt)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) l += fast_exp2(x[kt][i] - m);
+            l += __shfl_xor(l, 16, 64);
+            l += __shfl_xor(l, 32, 64);
+            const int buf = (c0 >> 4) & 1;   // (read before the next barrier, written again after it)
+            if (g == 0) {
+                ml[buf][w][c][0] = m;
+                ml[buf][w][c][1] = l;
+            }
+            lds_barrier();
+            if (w == 0 && g == 0 && valid) {
+                float M = ml[buf][0][c][0];
+#pragma unroll
+                for (int ww = 1; ww < kWaves; ++ww) M = fmaxf(M, ml[buf][ww][c][0]);
+                float S = 0.0f;
+#pragma unroll
+                for (int ww = 0; ww < kWaves; ++ww) S = fmaf(fast_exp2(ml[buf][ww][c][0] - M), ml[buf][ww][c][1], S);
+                a.part[qrow * a.nblk + blockIdx.x] = S == 0.0f ? -INFINITY : M + fast_log2(S);
+            }
+        }
+    }
+    if constexpr (SUM) {
+        float* mass = a.mass + n * a.mass_bs + kvh * a.mass_hs;
+#pragma unroll
+        for (int kt = 0; kt < KT; ++kt)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const float t = group_sum<16>(sum[kt][i]);
+                const int pos = p0[kt] + 4 * g + i;
+                if (c == 0 && pos < s.L) mass[pos] += t;
+            }
+    }
+}
+
+// Per column: the log2-sum-exp2 over its key blocks, +inf for a column that sees
+// no key (every weight is then zero).  Grid (rows of the longest window x Hq / 4, N), a wave per column.
+__global__ __launch_bounds__(256) void window_lse_kernel(WindowArgs a, int keys) {
+    const int n = blockIdx.y, lane = threadIdx.x & 63;
+    const WindowSeq s = window_seq(a, n);
+    const int nblk = (s.L + keys - 1) / keys;
+    for (int64_t r = blockIdx.x * 4 + (threadIdx.x >> 6); r < (int64_t)s.P * a.Hq; r += gridDim.x * 4) {
+        const int64_t at = (int64_t)s.q0 * a.Hq + r;
+        float M = -INFINITY, S = 0.0f;
+        for (int j = lane; j < nblk; j += 64) {
+            const float x = a.part[at * a.nblk + j];
+            const float mb = fmaxf(M, x);
+            if (mb == -INFINITY) continue;
+            S = S * fast_exp2(M - mb) + fast_exp2(x - mb);
+            M = mb;
+        }
+        const float top = wave_max(M);
+        S = wave_sum(top == -INFINITY ? 0.0f : S * fast_exp2(M - top));
+        if (lane == 0) a.lse[at] = S == 0.0f ? INFINITY : top + fast_log2(S);
+    }
+}
+
+// Any head_dim up to 256, any page size and alignment: a wave per (row, query
+// head) for the log-sum-exp, then a thread per (key, kv head) for the totals.
+template <typename T>
+__device__ inline float dot(const T* q, const T* k, int D) {
+    float d0 = 0.0f, d1 = 0.0f, d2 = 0.0f, d3 = 0.0f;   // four sums, added pairwise
+    int d = 0;
+    for (; d + 3 < D; d += 4) {
+        d0 = fmaf(Elem<T>::to_f32(q[d]), Elem<T>::to_f32(k[d]), d0);
+        d1 = fmaf(Elem<T>::to_f32(q[d + 1]), Elem<T>::to_f32(k[d + 1]), d1);
+        d2 = fmaf(Elem<T>::to_f32(q[d + 2]), Elem<T>::to_f32(k[d + 2]), d2);
+        d3 = fmaf(Elem<T>::to_f32(q[d + 3]), Elem<T>::to_f32(k[d + 3]), d3);
+    }
+    for (; d < D; ++d) d0 = fmaf(Elem<T>::to_f32(q[d]), Elem<T>::to_f32(k[d]), d0);
+    return (d0 + d1) + (d2 + d3);
+}
+
+template <typename T>
+__device__ inline const T* key_row(const WindowArgs& a, int n, int kvh, int pos) {
+    const int64_t phys = max(a.bt[(int64_t)n * a.max_blocks + pos / a.bs], 0);
+    return reinterpret_cast<const T*>(a.k) + ((phys * a.bs + pos % a.bs) * a.Hkv + kvh) * a.D;
+}
+
+template <typename T>
+__global__ __launch_bounds__(256) void window_lse_generic_kernel(WindowArgs a) {
+    const int n = blockIdx.y, lane = threadIdx.x & 63, G = a.Hq / a.Hkv;
+    const WindowSeq s = window_seq(a, n);
+    for (int64_t r = blockIdx.x * 4 + (threadIdx.x >> 6); r < (int64_t)s.P * a.Hq; r += gridDim.x * 4) {
+        const int64_t at = (int64_t)s.q0 * a.Hq + r;
+        const int node = (int)(r / a.Hq), kvh = (int)(r - (int64_t)node * a.Hq) / G;
+        const T* q = reinterpret_cast<const T*>(a.q) + at * a.D;
+        const int stop = min(s.hist + node + 1, s.L);
+        float M = -INFINITY, S = 0.0f;
+        for (int j = lane; j < stop; j += 64) {
+            const float x = dot(q, key_row<T>(a, n, kvh, j), a.D) * a.scale_log2;
+            const float mb = fmaxf(M, x);
+            if (mb == -INFINITY) continue;
+            S = S * fast_exp2(M - mb) + fast_exp2(x - mb);
+            M = mb;
+        }
+        const float top = wave_max(M);
+        S = wave_sum(top == -INFINITY ? 0.0f : S * fast_exp2(M - top));
+        if (lane == 0) a.lse[at] = S == 0.0f ? INFINITY : top + fast_log2(S);
+    }
+}
+
+template <typename T>
+__global__ __launch_bounds__(256) void window_sum_generic_kernel(WindowArgs a) {
+    const int n = blockIdx.z, kvh = blockIdx.y, G = a.Hq / a.Hkv;
+    const WindowSeq s = window_seq(a, n);
+    for (int j = blockIdx.x * 256 + threadIdx.x; j < s.L; j += gridDim.x * 256) {
+        const T* k = key_row<T>(a, n, kvh, j);
+        float sum = 0.0f;
+        for (int i = max(0, j - s.hist); i < s.P; ++i)
+            for (int h = 0; h < G; ++h) {
+                const int64_t at = (int64_t)(s.q0 + i) * a.Hq + kvh * G + h;
+                sum += fast_exp2(dot(reinterpret_cast<const T*>(a.q) + at * a.D, k, a.D) * a.scale_log2 - a.lse[at]);
+            }
+        a.mass[n * a.mass_bs + kvh * a.mass_hs + j] += sum;
+    }
+}
+
+bool tuned_shape(int D, int bs) { return bs == kPage && (D == 64 || D == 96 || D == 128 || D == 256); }
+
+int keys_of(int dtype) { return dtype == LLKV_DTYPE_F32 ? block_keys<float>() : block_keys<_Float16>(); }
+
+template <typename T, int D>
+void launch_tuned(const WindowArgs& a, int max_q_len, hipStream_t st) {
+    const dim3 grid(a.nblk, a.Hkv, a.N);
+    const int lse_wgs = (int)std::min<int64_t>(((int64_t)max_q_len * a.Hq + 3) / 4, 65535);
+    window_kernel<T, D, false><<<grid, 256, 0, st>>>(a);
+    window_lse_kernel<<<dim3(lse_wgs, a.N), 256, 0, st>>>(a, block_keys<T>());
+    window_kernel<T, D, true><<<grid, 256, 0, st>>>(a);
+}
+
+template <typename T>
+void launch_window(const WindowArgs& a, int max_q_len, bool tuned, hipStream_t st) {
+    if (tuned) {
+        if (a.D == 64) launch_tuned<T, 64>(a, max_q_len, st);
+        else if (a.D == 96) launch_tuned<T, 96>(a, max_q_len, st);
+        else if (a.D == 128) launch_tuned<T, 128>(a, max_q_len, st);
+        else launch_tuned<T, 256>(a, max_q_len, st);
+        return;
+    }
+    const int lse_wgs = (int)std::min<int64_t>(((int64_t)max_q_len * a.Hq + 3) / 4, 65535);
+    window_lse_generic_kernel<T><<<dim3(lse_wgs, a.N), 256, 0, st>>>(a);
+    const int blocks = std::max(1, std::min((a.max_len + 255) / 256, 65535));
+    window_sum_generic_kernel<T><<<dim3(blocks, a.Hkv, a.N), 256, 0, st>>>(a);
+}
+
+struct WindowPlan {
+    int nblk;
+    size_t lse, total;
+};
+
+WindowPlan window_plan(int64_t total_q, int Hq, int max_len, int dtype) {
+    WindowPlan p;
+    const int keys = keys_of(dtype);
+    p.nblk = (int)std::max<int64_t>(1, ((int64_t)max_len + keys - 1) / keys);
+    const size_t rows = (size_t)total_q * Hq * sizeof(float);
+    p.lse = (rows * p.nblk + 255) & ~(size_t)255;
+    p.total = p.lse + rows;
+    return p;
+}
+
+}  // namespace
+}  // namespace llkv
+
+using namespace llkv;
+
+extern "C" size_t llkv_paged_window_mass_workspace_size(int total_q, int num_q_heads, int max_seq_len, int dtype) {
+    if (total_q <= 0 || num_q_heads <= 0 || max_seq_len < 0 || dtype_bytes(dtype) == 0) return 0;
+    return window_plan(total_q, num_q_heads, max_seq_len, dtype).total;
+}
+
+extern "C" int llkv_paged_window_mass(float* mass, int64_t mass_seq_stride, int64_t mass_head_stride, const void* q,
+                                      const void* k_pool, const int* block_table, int max_blocks_per_seq,
+                                      const int* cu_q, const int* seq_lens, int num_seqs, int total_q, int max_q_len,
+                                      int max_seq_len, int num_q_heads, int num_kv_heads, int head_dim, int block_size,
+                                      float scale, int dtype, void* workspace, size_t workspace_bytes, void* stream) {
+    const char* fn = "llkv_paged_window_mass";
+    if (num_seqs == 0 || total_q == 0) return LLKV_OK;
+    if (num_seqs < 0 || total_q < 0 || max_q_len <= 0 || max_seq_len < 0 || num_q_heads <= 0 || num_kv_heads <= 0 ||
+        head_dim <= 0 || block_size <= 0 || max_blocks_per_seq <= 0)
+        return set_error(LLKV_ERR_INVALID, "%s: bad shape arguments", fn);
+    if (head_dim > 256) return set_error(LLKV_ERR_UNSUPPORTED, "%s: head_dim too large (%d > 256)", fn, head_dim);
+    if (num_q_heads % num_kv_heads != 0)
+        return set_error(LLKV_ERR_INVALID, "%s: num_q_heads %d not a multiple of num_kv_heads %d", fn, num_q_heads,
+                         num_kv_heads);
+    if (dtype_bytes(dtype) == 0) return set_error(LLKV_ERR_INVALID, "%s: unsupported dtype %d", fn, dtype);
+    if ((int64_t)max_blocks_per_seq * block_size > INT32_MAX - 1024 || (int64_t)num_seqs * max_blocks_per_seq > INT32_MAX ||
+        num_kv_heads > 65535 || (int64_t)total_q * num_q_heads > INT32_MAX - 256)
+        return set_error(LLKV_ERR_UNSUPPORTED, "%s: block table or rows too large", fn);
+    if (!mass || !q || !k_pool || !block_table || !cu_q || !seq_lens)
+        return set_error(LLKV_ERR_INVALID, "%s: null pointer", fn);
+    if (mass_head_stride < max_seq_len || (num_seqs > 1 && mass_seq_stride < (int64_t)num_kv_heads * mass_head_stride))
+        return set_error(LLKV_ERR_INVALID, "%s: totals of %lld keys a head for up to %d", fn,
+                         (long long)mass_head_stride, max_seq_len);
+    const WindowPlan p = window_plan(total_q, num_q_heads, max_seq_len, dtype);
+    if (!workspace || workspace_bytes < p.total)
+        return set_error(LLKV_ERR_WORKSPACE, "%s: workspace of %zu bytes, %zu needed", fn, workspace_bytes, p.total);
+    if (((uintptr_t)workspace & 15) != 0) return set_error(LLKV_ERR_INVALID, "%s: workspace not 16-byte aligned", fn);
+    WindowArgs a = {};
+    a.q = q;
+    a.k = k_pool;
+    a.cu_q = cu_q;
+    a.max_blocks = max_blocks_per_seq;
+    a.Hq = num_q_heads;
+    a.Hkv = num_kv_heads;
+    a.D = head_dim;
+    a.bs = block_size;
+    a.max_len = max_seq_len;
+    a.scale_log2 = scale * kLog2e;
+    a.nblk = p.nblk;
+    a.part = reinterpret_cast<float*>(workspace);
+    a.lse = reinterpret_cast<float*>(reinterpret_cast<char*>(workspace) + p.lse);
+    a.mass_bs = mass_seq_stride;
+    a.mass_hs = mass_head_stride;
+    const bool tuned = tuned_shape(head_dim, block_size) && (((uintptr_t)q | (uintptr_t)k_pool) & 15) == 0;
+    hipStream_t st = (hipStream_t)stream;
+    constexpr int kMost = 32768;   // sequences per launch (a grid's extent in z)
+    for (int n0 = 0; n0 < num_seqs; n0 += kMost) {
+        a.N = std::min(num_seqs - n0, kMost);
+        a.bt = block_table + (int64_t)n0 * max_blocks_per_seq;
+        a.cu_q = cu_q + n0;
+        a.lens = seq_lens + n0;
+        a.mass = mass + n0 * mass_seq_stride;
+        if (dtype == LLKV_DTYPE_F32) launch_window<float>(a, max_q_len, tuned, st);
+        else if (dtype == LLKV_DTYPE_F16) launch_window<_Float16>(a, max_q_len, tuned, st);
+        else launch_window<bf16_t>(a, max_q_len, tuned, st);
+    }
+    return check_launch(fn);
+}

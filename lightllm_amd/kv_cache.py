@@ -11,7 +11,7 @@ from __future__ import annotations
 import ctypes
 import functools
 import math
-from typing import Optional, Sequence
+from typing import Optional, Sequence, Union
 
 import torch
 
@@ -438,3 +438,336 @@ def first_prefill_attn_batched(out: torch.Tensor, q: torch.Tensor, k: torch.Tens
                                            _ptr(offsets), _ptr(kv_offsets), _ptr(num_tokens),
                                            _ptr(token_cumsum), _ptr(start_poss), n, p_total, max_tokens,
                                            scale, dtype_code(q.dtype), _stream(stream)))
+
+
+# ---------------------------------------------------------------------------
+# The cache step's further operators: norm + rotation + append, drafted trees, accumulated weights
+# and eviction.  Their arguments are checked in full (device, type, shape), before anything is
+# launched.  Workspaces and outputs come from torch's allocator on the stream of the call, so that
+# calls on different streams share none, and a captured call owns its own.
+# ---------------------------------------------------------------------------
+
+def _device_of(pool: torch.Tensor) -> int:
+    """The device of a call: the pool's, which has to be the current one."""
+    if not pool.is_cuda:
+        raise ValueError("the pools must be on a GPU")
+    index = pool.device.index
+    if index != torch._C._cuda_getDevice():
+        raise ValueError(f"the pools are on cuda:{index}, which is not the current device")
+    return index
+
+
+def _check(t: torch.Tensor, dtype: torch.dtype, shape: tuple, device: int, name: str):
+    """`t` is contiguous, of this type, on this device, with this shape (None: any extent)."""
+    _require(t, dtype, name)
+    if t.dim() != len(shape) or any(n is not None and n != m for n, m in zip(shape, t.shape)):
+        raise ValueError(f"{name}: expected shape {shape}, got {tuple(t.shape)}")
+    if t.get_device() != device:
+        raise ValueError(f"{name}: must be on cuda:{device}")
+
+
+def _check_pools(k_pool: torch.Tensor, v_pool: Optional[torch.Tensor]):
+    device = _device_of(k_pool)
+    dtype_code(k_pool.dtype)
+    _check(k_pool, k_pool.dtype, (None,) * 4, device, "k_pool")
+    if v_pool is not None:
+        _check(v_pool, k_pool.dtype, tuple(k_pool.shape), device, "v_pool")
+    return device
+
+
+def _check_rows(t: torch.Tensor, dtype: torch.dtype, shape: tuple, device: int, name: str) -> int:
+    """Rows [T, heads, D] whose heads are contiguous; returns the elements between tokens."""
+    if t.dtype != dtype:
+        raise TypeError(f"{name}: expected {dtype}, got {t.dtype}")
+    if tuple(t.shape) != shape:
+        raise ValueError(f"{name}: expected shape {shape}, got {tuple(t.shape)}")
+    if t.numel() and (t.stride(2) != 1 and t.shape[2] > 1 or t.stride(1) != t.shape[2] and t.shape[1] > 1):
+        raise ValueError(f"{name}: the heads of a token must be contiguous")
+    if t.get_device() != device:
+        raise ValueError(f"{name}: must be on cuda:{device}")
+    return t.stride(0)
+
+
+def _check_mass(mass: torch.Tensor, n: int, hkv: int, device: int, name: str = "mass"):
+    """Totals [N, Hkv, width] with contiguous rows of keys; returns their strides."""
+    if mass.dtype != torch.float32:
+        raise TypeError(f"{name}: expected torch.float32, got {mass.dtype}")
+    if mass.dim() != 3 or mass.shape[0] != n or mass.shape[1] != hkv:
+        raise ValueError(f"{name}: expected shape ({n}, {hkv}, keys), got {tuple(mass.shape)}")
+    if mass.get_device() != device:
+        raise ValueError(f"{name}: must be on cuda:{device}")
+    width = mass.shape[2]
+    bs, hs, ks = mass.stride()
+    if hkv == 1:
+        hs = width
+    if n == 1:
+        bs = hkv * hs
+    if ks != 1 and width > 1 or hs < width or bs < hkv * hs:
+        raise ValueError(f"{name}: rows of keys must be contiguous and must not overlap")
+    return bs, hs
+
+
+def _empty(shape: tuple, dtype: torch.dtype, device: int, stream) -> torch.Tensor:
+    """A tensor of the call's stream (memory that another stream still uses is not handed out)."""
+    if stream is None:
+        return torch.empty(shape, dtype=dtype, device=torch.device("cuda", device))
+    with torch.cuda.stream(stream):
+        return torch.empty(shape, dtype=dtype, device=torch.device("cuda", device))
+
+
+def _scratch(nbytes: int, given: Optional[torch.Tensor], device: int, stream):
+    """(address, bytes) of a workspace: the caller's, or one from torch's allocator, returned as the
+    third value to be held until the call is enqueued."""
+    if given is not None:
+        if given.get_device() != device:
+            raise ValueError(f"workspace: must be on cuda:{device}")
+        if not given.is_contiguous():
+            raise ValueError("workspace: must be contiguous")
+        return given.data_ptr(), given.numel() * given.element_size(), given
+    if nbytes == 0:
+        return None, 0, None
+    ws = _empty((nbytes,), torch.uint8, device, stream)
+    return ws.data_ptr(), nbytes, ws
+
+
+def _scale(scale: Optional[float], d: int) -> float:
+    return 1.0 / math.sqrt(d) if scale is None else scale
+
+
+def qk_norm_rope_append(q: Optional[torch.Tensor], k: torch.Tensor, v: torch.Tensor, slot_mapping: torch.Tensor,
+                        positions: torch.Tensor, inv_freq: torch.Tensor, k_pool: torch.Tensor,
+                        v_pool: torch.Tensor, q_weight: Optional[torch.Tensor] = None,
+                        k_weight: Optional[torch.Tensor] = None, eps: float = 1e-6,
+                        pair_axis: Optional[Union[bytes, Sequence[int]]] = None,
+                        q_out: Optional[torch.Tensor] = None, k_out: Optional[torch.Tensor] = None,
+                        stream=None) -> Optional[torch.Tensor]:
+    """RMS norm of every query and key head (fp32 weights [D], or None), rotation of the first
+    2 * len(inv_freq) dims (Neox halves) and KV append, in one pass; returns q_out.
+
+    q [T, Hq, D] (or None), k and v [T, Hkv, D]: heads contiguous, any distance between tokens (slices
+    of a fused projection).  positions: int32 [T] or [axes, T], up to four axes; pair_axis: the axis of
+    each rotated pair, len(inv_freq) small integers (host; not needed with one axis).  inv_freq: fp32.
+    q_out: a new tensor by default; q itself rotates in place.  k_out: None writes the k rows to the
+    pool only.  The k and v rows go to pool rows slot_mapping[t] (<0 skips)."""
+    device = _check_pools(k_pool, v_pool)
+    hkv, d = k_pool.shape[2], k_pool.shape[3]
+    if k.dim() != 3:
+        raise ValueError(f"k: expected 3 dims, got {k.dim()}")
+    dt, t = k_pool.dtype, k.shape[0]
+    ks = _check_rows(k, dt, (t, hkv, d), device, "k")
+    vs = _check_rows(v, dt, (t, hkv, d), device, "v")
+    _check(slot_mapping, torch.int64, (t,), device, "slot_mapping")
+    if positions.dim() == 1:
+        positions = positions[None]
+    _check(positions, torch.int32, (None, t), device, "positions")
+    _check(inv_freq, torch.float32, (None,), device, "inv_freq")
+    for name, w in (("q_weight", q_weight), ("k_weight", k_weight)):
+        if w is not None:
+            _check(w, torch.float32, (d,), device, name)
+    axes, half = positions.shape[0], inv_freq.shape[0]
+    if pair_axis is not None:
+        if not isinstance(pair_axis, bytes):
+            pair_axis = bytes(pair_axis)
+        if len(pair_axis) != half:
+            raise ValueError(f"pair_axis: {len(pair_axis)} axes for {half} pairs")
+        if half and max(pair_axis) >= axes:
+            raise ValueError(f"pair_axis: axis {max(pair_axis)} of {axes}")
+    hq = qs = qos = kos = 0
+    if q is not None:
+        if q.dim() != 3:
+            raise ValueError(f"q: expected 3 dims, got {q.dim()}")
+        hq = q.shape[1]
+        qs = _check_rows(q, dt, (t, hq, d), device, "q")
+        if q_out is None:
+            q_out = _empty((t, hq, d), dt, device, stream)
+        qos = _check_rows(q_out, dt, (t, hq, d), device, "q_out")
+    elif q_out is not None:
+        raise ValueError("q_out: there is no q")
+    if k_out is not None:
+        kos = _check_rows(k_out, dt, (t, hkv, d), device, "k_out")
+    check(lib().llkv_qk_norm_rope_append(
+        _ptr(q_out), _ptr(k_out), _ptr(q), _ptr(k), _ptr(v), qos, kos, qs, ks, vs, _ptr(k_pool), _ptr(v_pool),
+        _ptr(slot_mapping), _ptr(positions), axes, pair_axis, _ptr(inv_freq), _ptr(q_weight), _ptr(k_weight), eps,
+        t, hq, hkv, d, 2 * half, dtype_code(dt), _stream(stream)))
+    return q_out
+
+
+def build_tree(parents: torch.Tensor, cu_q: torch.Tensor, seq_lens: torch.Tensor, max_q_len: int,
+               tree_mask: Optional[torch.Tensor] = None, positions: Optional[torch.Tensor] = None, stream=None):
+    """(tree_mask int32 [total_q, words], positions int32 [total_q]) of drafted trees: parents int32
+    [total_q] within each sequence's rows cu_q[n]:cu_q[n+1], anything outside [0, i) a root; the mask has
+    node i itself and its ancestors, the position is the context's length plus the depth."""
+    if not parents.is_cuda:
+        raise ValueError("parents: must be on a GPU")
+    device = _device_of(parents)
+    n, total = seq_lens.shape[0], parents.shape[0]
+    _check(parents, torch.int32, (total,), device, "parents")
+    _check(seq_lens, torch.int32, (n,), device, "seq_lens")
+    _check(cu_q, torch.int32, (n + 1,), device, "cu_q")
+    if tree_mask is None:
+        tree_mask = _empty((total, (max_q_len + 31) // 32), torch.int32, device, stream)
+    if positions is None:
+        positions = _empty((total,), torch.int32, device, stream)
+    _check(tree_mask, torch.int32, (total, None), device, "tree_mask")
+    _check(positions, torch.int32, (total,), device, "positions")
+    check(lib().llkv_build_tree(_ptr(tree_mask), tree_mask.shape[1], _ptr(positions), _ptr(parents), _ptr(cu_q),
+                                _ptr(seq_lens), n, total, max_q_len, _stream(stream)))
+    return tree_mask, positions
+
+
+@functools.lru_cache(maxsize=256)
+def _tree_size(*shape: int) -> int:
+    return lib().llkv_paged_tree_attention_workspace_size(*shape)
+
+
+@functools.lru_cache(maxsize=256)
+def _mass_size(*shape: int) -> int:
+    return lib().llkv_paged_decode_mass_workspace_size(*shape)
+
+
+def paged_tree_attention(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor, block_table: torch.Tensor,
+                         cu_q: torch.Tensor, seq_lens: torch.Tensor, tree_mask: torch.Tensor, max_q_len: int,
+                         max_seq_len: int, scale: Optional[float] = None, out: Optional[torch.Tensor] = None,
+                         workspace: Optional[torch.Tensor] = None, stream=None) -> torch.Tensor:
+    """Attention of drafted trees: q [total_q, Hq, D], sequence n owning rows cu_q[n]:cu_q[n+1], whose K
+    and V are its last cached positions.  A row sees the whole context and the nodes j of its sequence
+    whose bit is set in its row of tree_mask (int32 [total_q, words]; build_tree)."""
+    device = _check_pools(k_pool, v_pool)
+    _, bs, hkv, d = k_pool.shape
+    tq, hq = q.shape[0], q.shape[1]
+    n = seq_lens.shape[0]
+    _check(q, k_pool.dtype, (tq, hq, d), device, "q")
+    _check(seq_lens, torch.int32, (n,), device, "seq_lens")
+    _check(block_table, torch.int32, (n, None), device, "block_table")
+    _check(cu_q, torch.int32, (n + 1,), device, "cu_q")
+    _check(tree_mask, torch.int32, (tq, None), device, "tree_mask")
+    if out is None:
+        out = _empty(tuple(q.shape), q.dtype, device, stream)
+    _check(out, k_pool.dtype, tuple(q.shape), device, "out")
+    max_q_len, max_seq_len, dt = int(max_q_len), int(max_seq_len), dtype_code(q.dtype)
+    ws, nbytes, held = _scratch(_tree_size(n, max_q_len, hq, hkv, d, bs, max_seq_len, dt), workspace, device, stream)
+    check(lib().llkv_paged_tree_attention(_ptr(out), _ptr(q), _ptr(k_pool), _ptr(v_pool), _ptr(block_table),
+                                          block_table.shape[1], _ptr(cu_q), _ptr(seq_lens), _ptr(tree_mask),
+                                          tree_mask.shape[1], n, tq, max_q_len, max_seq_len, hq, hkv, d, bs,
+                                          _scale(scale, d), dt, ws, nbytes, _stream(stream)))
+    return out
+
+
+def paged_decode_mass(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor, block_table: torch.Tensor,
+                      seq_lens: torch.Tensor, max_seq_len: int, mass: torch.Tensor, scale: Optional[float] = None,
+                      out: Optional[torch.Tensor] = None, workspace: Optional[torch.Tensor] = None,
+                      stream=None) -> torch.Tensor:
+    """paged_decode that also adds each key's weight, summed over the query heads of its kv head, to
+    mass: fp32 [B, Hkv, keys >= max_seq_len]."""
+    device = _check_pools(k_pool, v_pool)
+    _, bs, hkv, d = k_pool.shape
+    b, hq = q.shape[0], q.shape[1]
+    _check(q, k_pool.dtype, (b, hq, d), device, "q")
+    _check(seq_lens, torch.int32, (b,), device, "seq_lens")
+    _check(block_table, torch.int32, (b, None), device, "block_table")
+    mass_bs, mass_hs = _check_mass(mass, b, hkv, device)
+    max_seq_len, dt = int(max_seq_len), dtype_code(q.dtype)
+    if mass.shape[2] < max_seq_len:
+        raise ValueError(f"mass: rows of {mass.shape[2]} keys for up to {max_seq_len}")
+    if out is None:
+        out = _empty(tuple(q.shape), q.dtype, device, stream)
+    _check(out, k_pool.dtype, tuple(q.shape), device, "out")
+    ws, nbytes, held = _scratch(_mass_size(b, hq, hkv, d, bs, max_seq_len, dt), workspace, device, stream)
+    check(lib().llkv_paged_decode_mass(_ptr(out), _ptr(mass), mass_bs, mass_hs, _ptr(q), _ptr(k_pool), _ptr(v_pool),
+                                       _ptr(block_table), _ptr(seq_lens), b, hq, hkv, d, bs, block_table.shape[1],
+                                       max_seq_len, _scale(scale, d), dt, ws, nbytes, _stream(stream)))
+    return out
+
+
+def paged_window_mass(q: torch.Tensor, k_pool: torch.Tensor, block_table: torch.Tensor, cu_q: torch.Tensor,
+                      seq_lens: torch.Tensor, max_q_len: int, max_seq_len: int, mass: torch.Tensor,
+                      scale: Optional[float] = None, workspace: Optional[torch.Tensor] = None, stream=None) -> None:
+    """Adds the weights that the last rows of each sequence (q [total_q, Hq, D], rows
+    cu_q[n]:cu_q[n+1] its last tokens, causal) give to each of its keys to mass, fp32 [N, Hkv,
+    keys >= max_seq_len]."""
+    device = _check_pools(k_pool, None)
+    _, bs, hkv, d = k_pool.shape
+    tq, hq = q.shape[0], q.shape[1]
+    n = seq_lens.shape[0]
+    _check(q, k_pool.dtype, (tq, hq, d), device, "q")
+    _check(seq_lens, torch.int32, (n,), device, "seq_lens")
+    _check(block_table, torch.int32, (n, None), device, "block_table")
+    _check(cu_q, torch.int32, (n + 1,), device, "cu_q")
+    mass_bs, mass_hs = _check_mass(mass, n, hkv, device)
+    max_q_len, max_seq_len, dt = int(max_q_len), int(max_seq_len), dtype_code(q.dtype)
+    if mass.shape[2] < max_seq_len:
+        raise ValueError(f"mass: rows of {mass.shape[2]} keys for up to {max_seq_len}")
+    need = lib().llkv_paged_window_mass_workspace_size(tq, hq, max_seq_len, dt)
+    ws, nbytes, held = _scratch(need, workspace, device, stream)
+    check(lib().llkv_paged_window_mass(_ptr(mass), mass_bs, mass_hs, _ptr(q), _ptr(k_pool), _ptr(block_table),
+                                       block_table.shape[1], _ptr(cu_q), _ptr(seq_lens), n, tq, max_q_len,
+                                       max_seq_len, hq, hkv, d, bs, _scale(scale, d), dt, ws, nbytes,
+                                       _stream(stream)))
+
+
+def evict_select(mass: torch.Tensor, seq_lens: torch.Tensor, budget: int, max_seq_len: int, sinks: int = 0,
+                 recent: int = 0, stream=None):
+    """(keep int32 [N, Hkv, budget], counts int32 [N], totals like mass): for every kv head the positions to
+    keep, rising, -1 behind the last: the first `sinks`, the last `recent`, and the largest totals of the rest
+    (ties: the lower position); the kept totals in the same order, zeros behind them."""
+    device = _device_of(mass)
+    n, hkv = mass.shape[0], mass.shape[1]
+    mass_bs, mass_hs = _check_mass(mass, n, hkv, device)
+    _check(seq_lens, torch.int32, (n,), device, "seq_lens")
+    max_seq_len, width = int(max_seq_len), mass.shape[2]
+    if width < max_seq_len:
+        raise ValueError(f"mass: rows of {width} keys for up to {max_seq_len}")
+    if budget <= 0 or sinks < 0 or recent < 0 or sinks + recent > budget:
+        raise ValueError(f"a budget of {budget} for {sinks} sinks and {recent} recent keys")
+    keep = _empty((n, hkv, budget), torch.int32, device, stream)
+    counts = _empty((n,), torch.int32, device, stream)
+    out = _empty((n, hkv, width), torch.float32, device, stream)
+    check(lib().llkv_evict_select(_ptr(keep), _ptr(counts), _ptr(out), hkv * width, width, width, _ptr(mass), mass_bs,
+                                  mass_hs, _ptr(seq_lens), n, hkv, max_seq_len, budget, sinks, recent,
+                                  _stream(stream)))
+    return keep, counts, out
+
+
+def compact_kv(k_pool: torch.Tensor, v_pool: torch.Tensor, block_table: torch.Tensor, keep: torch.Tensor,
+               counts: torch.Tensor, dst_table: Optional[torch.Tensor] = None,
+               dst_start: Optional[torch.Tensor] = None, stream=None) -> None:
+    """Moves the K and V rows at positions keep[n, h, i], i < counts[n] (keep int32 [N, Hkv or 1, M]; 1: all
+    heads alike) to positions dst_start[n] + i (0 + i): of dst_table's pages, which hold none of the rows
+    read, or in place (dst_table None; keep rising, keep[i] >= dst_start + i, and pages that no other
+    sequence shares)."""
+    device = _check_pools(k_pool, v_pool)
+    _, bs, hkv, d = k_pool.shape
+    n = block_table.shape[0]
+    _check(block_table, torch.int32, (n, None), device, "block_table")
+    _check(counts, torch.int32, (n,), device, "counts")
+    if keep.dim() != 3 or keep.shape[1] not in (1, hkv):
+        raise ValueError(f"keep: expected shape ({n}, {hkv} or 1, positions), got {tuple(keep.shape)}")
+    _check(keep, torch.int32, (n, None, None), device, "keep")
+    if dst_table is not None:
+        _check(dst_table, torch.int32, (n, None), device, "dst_table")
+    if dst_start is not None:
+        _check(dst_start, torch.int32, (n,), device, "dst_start")
+    check(lib().llkv_compact(_ptr(k_pool), _ptr(v_pool), _ptr(block_table), block_table.shape[1], _ptr(dst_table),
+                             dst_table.shape[1] if dst_table is not None else 0, _ptr(keep), keep.shape[1],
+                             keep.shape[2], _ptr(counts), _ptr(dst_start), n, hkv, d, bs, dtype_code(k_pool.dtype),
+                             _stream(stream)))
+
+
+def evict_kv(k_pool: torch.Tensor, v_pool: torch.Tensor, block_table: torch.Tensor, seq_lens: torch.Tensor,
+             mass: torch.Tensor, budget: int, max_seq_len: int, sinks: int = 0, recent: int = 0,
+             dst_table: Optional[torch.Tensor] = None, stream=None):
+    """Cuts every sequence down to at most `budget` keys per kv head by their totals (evict_select) and moves
+    their rows (compact_kv) to positions 0 .. of dst_table's pages, or of its own with dst_table None.
+    Returns (keep, counts, totals): counts are the new lengths.  The rows keep the rotation of their old
+    positions, and new tokens go on with theirs; the caller frees what the tables no longer need."""
+    device = _check_pools(k_pool, v_pool)
+    n = seq_lens.shape[0]
+    _check_mass(mass, n, k_pool.shape[2], device)
+    _check(block_table, torch.int32, (n, None), device, "block_table")
+    if dst_table is not None:
+        _check(dst_table, torch.int32, (n, None), device, "dst_table")
+        if dst_table.shape[1] * k_pool.shape[1] < min(budget, int(max_seq_len)):
+            raise ValueError(f"dst_table: {dst_table.shape[1]} pages for {budget} keys")
+    keep, counts, totals = evict_select(mass, seq_lens, budget, max_seq_len, sinks, recent, stream)
+    compact_kv(k_pool, v_pool, block_table, keep, counts, dst_table, stream=stream)
+    return keep, counts, totals
