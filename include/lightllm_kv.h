@@ -388,12 +388,15 @@ int llkv_paged_window_mass(float* mass, int64_t mass_seq_stride, int64_t mass_he
  * with the largest totals, ties going to the lower position; a NaN total is
  * below every number.  mass_out (rows of out_width >= min(budget, max_seq_len)
  * values; not overlapping mass) gets the kept totals in the same order, then
- * zeros.  seq_lens beyond max_seq_len are cut off at it. */
+ * zeros.  seq_lens beyond max_seq_len are cut off at it.  workspace:
+ * llkv_evict_select_workspace_size() bytes, 16-byte aligned, uninitialised (may
+ * be NULL when that size is 0); calls that share it must not overlap. */
+size_t llkv_evict_select_workspace_size(int num_seqs, int num_kv_heads, int max_seq_len);
 int llkv_evict_select(int* keep, int* counts, float* mass_out, int64_t out_seq_stride,
                       int64_t out_head_stride, int out_width, const float* mass,
                       int64_t mass_seq_stride, int64_t mass_head_stride, const int* seq_lens,
                       int num_seqs, int num_kv_heads, int max_seq_len, int budget, int sinks,
-                      int recent, void* stream);
+                      int recent, void* workspace, size_t workspace_bytes, void* stream);
 
 /* Moves rows of K and V, bit for bit: position keep[n][h][i] of sequence n (of
  * kv head h; keep_heads 1: of all heads) to position dst_start[n] + i

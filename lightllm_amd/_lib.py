@@ -55,8 +55,9 @@ _SIGS = {
     "llkv_paged_window_mass_workspace_size": (c_size_t, [c_int] * 4),
     "llkv_paged_window_mass": (c_int, [c_void_p, c_int64, c_int64] + [c_void_p] * 3 + [c_int] + [c_void_p] * 2
                                + [c_int] * 8 + [c_float, c_int, c_void_p, c_size_t, c_void_p]),
+    "llkv_evict_select_workspace_size": (c_size_t, [c_int] * 3),
     "llkv_evict_select": (c_int, [c_void_p] * 3 + [c_int64, c_int64, c_int, c_void_p, c_int64, c_int64, c_void_p]
-                          + [c_int] * 6 + [c_void_p]),
+                          + [c_int] * 6 + [c_void_p, c_size_t, c_void_p]),
     "llkv_compact": (c_int, [c_void_p] * 3 + [c_int, c_void_p, c_int, c_void_p, c_int, c_int, c_void_p, c_void_p]
                      + [c_int] * 5 + [c_void_p]),
     "llkv_paged_decode_workspace_size": (c_size_t, [c_int, c_int, c_int, c_int, c_int, c_int, c_int]),

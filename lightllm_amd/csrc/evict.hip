@@ -23,6 +23,12 @@ namespace {
 
 constexpr int kSelThreads = 1024;
 constexpr int kSelWaves = kSelThreads / 64;
+constexpr int kBins = 2048;          // of a digit: two per thread
+constexpr int kOnePass = 16;         // keys per thread of the one-launch form, at most
+constexpr int kChunk = 8 * kSelThreads;   // keys per work-group of the other
+
+// The three digits of a rank, from the top.
+constexpr int kShift[3] = {21, 10, 0};
 
 struct SelectArgs {
     const float* mass;
@@ -33,116 +39,293 @@ struct SelectArgs {
     int64_t mass_bs, mass_hs, out_bs, out_hs;
     int width;        // of mass_out's rows
     int budget, sinks, recent, max_len, Hkv;
+    // Keys in chunks (max_len > kOnePass * kSelThreads): per (sequence, kv head, chunk) the
+    // digit histograms, 16 bits a bin, of the first and third digit and of the second, and
+    // the number of keys above the threshold by the first and by the second digit.
+    int chunks;
+    uint32_t* hist[2];   // [units][chunks][kBins / 2]
+    int* above[2];       // [units][chunks]
+    int* found;          // [units][4]: (digits so far, keys left) after the first and the second digit
 };
 
 // Unsigned image of a total: larger totals are larger integers, the two zeros
 // are equal, NaN is below everything, and 0xFFFFFFFF is above every total.
 __device__ inline uint32_t rank_of(float x) {
-    if (x != x) return 0u;
     const uint32_t b = __float_as_uint(x + 0.0f);
-    return (b & 0x80000000u) ? ~b : (b | 0x80000000u);
+    const uint32_t r = (b & 0x80000000u) ? ~b : (b | 0x80000000u);
+    return x != x ? 0u : r;
 }
 
-__device__ inline uint32_t rank_at(const SelectArgs& a, const float* mass, int j, int L) {
-    if (j < a.sinks || j >= L - a.recent) return 0xFFFFFFFFu;
-    return rank_of(mass[j]);
+struct Unit {
+    int n, kvh, L, count;
+    const float* mass;
+    float* out;
+    int* keep;
+    int64_t index;
+};
+
+__device__ inline Unit unit_of(const SelectArgs& a, int kvh, int n) {
+    Unit u;
+    const int len = a.lens[n];
+    u.n = n;
+    u.kvh = kvh;
+    u.L = len < 0 ? 0 : (len > a.max_len ? a.max_len : len);
+    u.count = min(u.L, a.budget);
+    u.mass = a.mass + n * a.mass_bs + kvh * a.mass_hs;
+    u.out = a.mass_out + n * a.out_bs + kvh * a.out_hs;
+    u.index = (int64_t)n * a.Hkv + kvh;
+    u.keep = a.keep + u.index * a.budget;
+    return u;
 }
 
-// Grid (Hkv, N).
-__global__ __launch_bounds__(kSelThreads) void select_kernel(SelectArgs a) {
-    __shared__ int hist[256];
-    __shared__ int s_digit, s_left;
-    __shared__ int s_above[kSelWaves], s_equal[kSelWaves];
-    const int kvh = blockIdx.x, n = blockIdx.y, tid = threadIdx.x, lane = tid & 63, wv = tid >> 6;
-    const int len = a.lens[n], L = len < 0 ? 0 : (len > a.max_len ? a.max_len : len);
-    const int count = min(L, a.budget);
-    const float* mass = a.mass + n * a.mass_bs + kvh * a.mass_hs;
-    float* out = a.mass_out + n * a.out_bs + kvh * a.out_hs;
-    int* keep = a.keep + ((int64_t)n * a.Hkv + kvh) * a.budget;
-    if (kvh == 0 && tid == 0) a.counts[n] = count;
-    for (int i = count + tid; i < a.budget; i += kSelThreads) keep[i] = -1;
-    for (int i = count + tid; i < a.width; i += kSelThreads) out[i] = 0.0f;
-    if (L <= a.budget) {   // uniform
-        for (int i = tid; i < count; i += kSelThreads) {
-            keep[i] = i;
-            out[i] = mass[i];
+// Ranks of the keys j0 + 1024 e + thread, 0 beyond the unit's last (with `valid` cleared).
+template <int VPT>
+struct Ranks {
+    uint32_t r[VPT];
+    uint32_t valid;
+
+    __device__ inline void load(const SelectArgs& a, const Unit& u, int j0) {
+        valid = 0;
+        float x[VPT];
+#pragma unroll
+        for (int e = 0; e < VPT; ++e) {
+            const int j = j0 + e * kSelThreads + (int)threadIdx.x;
+            x[e] = u.mass[min(j, u.L - 1)];
         }
+#pragma unroll
+        for (int e = 0; e < VPT; ++e) {
+            const int j = j0 + e * kSelThreads + (int)threadIdx.x;
+            r[e] = (j < a.sinks || j >= u.L - a.recent) ? 0xFFFFFFFFu : rank_of(x[e]);
+            valid |= (uint32_t)(j < u.L) << e;
+        }
+    }
+
+    // Whether key e has the digits of `prefix` above digit `pass`.
+    __device__ inline bool matches(int e, int pass, uint32_t prefix) const {
+        return pass == 0 || (r[e] >> kShift[pass - 1]) == (prefix >> kShift[pass - 1]);
+    }
+
+    // Adds the digits `pass` of the keys whose digits above are those of `prefix`.  Totals
+    // crowd in few bins of the first digit (equal ones in one bin of each): a wave whose
+    // keys share a bin adds once.
+    __device__ inline void histogram(int* hist, int pass, uint32_t prefix) const {
+        const int shift = pass == 0 ? kShift[0] : (pass == 1 ? kShift[1] : kShift[2]);
+        const int bits = pass == 2 ? 10 : 11;
+#pragma unroll
+        for (int e = 0; e < VPT; ++e) {
+            const bool in = (valid >> e & 1u) && matches(e, pass, prefix);
+            const int d = (int)(r[e] >> shift) & ((1 << bits) - 1);
+            const uint64_t act = __builtin_amdgcn_ballot_w64(in);
+            if (act == 0) continue;
+            const int first = __builtin_ctzll(act);
+            const int d0 = __builtin_amdgcn_readlane(d, first);
+            if (__builtin_amdgcn_ballot_w64(in && d == d0) == act) {
+                if ((int)(threadIdx.x & 63) == first) atomicAdd(&hist[d0], __builtin_popcountll(act));
+            } else if (in) {
+                atomicAdd(&hist[d], 1);
+            }
+        }
+    }
+};
+
+struct SelectSmem {
+    int hist[kBins];
+    int wave_sum[kSelWaves];
+    int digit, left;
+    int gt[kOnePass * kSelWaves], eq[kOnePass * kSelWaves];
+};
+
+__device__ inline int wave_scan(int v) {
+    const int lane = threadIdx.x & 63;
+#pragma unroll
+    for (int off = 1; off < 64; off <<= 1) {
+        const int t = __shfl_up(v, off, 64);
+        if (lane >= off) v += t;
+    }
+    return v;
+}
+
+// The digit at which the `left` largest end: thread t holds the numbers hi and lo
+// of bins 2047 - 2t and 2046 - 2t.  Every thread gets the digit, how many of its
+// bin are kept.
+__device__ inline void find_digit(SelectSmem& s, int hi, int lo, int left, int& digit, int& keep) {
+    const int lane = threadIdx.x & 63, wv = threadIdx.x >> 6;
+    const int incl = wave_scan(hi + lo);
+    if (lane == 63) s.wave_sum[wv] = incl;
+    __syncthreads();
+    int before = incl - hi - lo;
+    for (int i = 0; i < wv; ++i) before += s.wave_sum[i];
+    const int bin = kBins - 1 - 2 * (int)threadIdx.x;
+    if (before < left && before + hi >= left) {
+        s.digit = bin;
+        s.left = left - before;
+    } else if (before + hi < left && before + hi + lo >= left) {
+        s.digit = bin - 1;
+        s.left = left - before - hi;
+    }
+    __syncthreads();
+    digit = s.digit;
+    keep = s.left;
+    __syncthreads();
+}
+
+// Writes the kept keys of these ranks: those above the threshold and, of the ones
+// equal to it, the first `left`, ga and ea of which lie in earlier chunks.
+template <int VPT>
+__device__ inline void write_kept(const SelectArgs& a, const Unit& u, SelectSmem& s, const Ranks<VPT>& k, int j0,
+                                  uint32_t threshold, int left, int ga, int ea) {
+    const int lane = threadIdx.x & 63, wv = threadIdx.x >> 6;
+#pragma unroll
+    for (int e = 0; e < VPT; ++e) {
+        const bool valid = k.valid >> e & 1u;
+        const uint64_t bg = __builtin_amdgcn_ballot_w64(valid && k.r[e] > threshold);
+        const uint64_t be = __builtin_amdgcn_ballot_w64(valid && k.r[e] == threshold);
+        if (lane == 0) {
+            s.gt[e * kSelWaves + wv] = __builtin_popcountll(bg);
+            s.eq[e * kSelWaves + wv] = __builtin_popcountll(be);
+        }
+    }
+    __syncthreads();
+    if (wv < 2) {   // exclusive prefix sums in the order of the positions
+        int* list = wv == 0 ? s.gt : s.eq;
+        int run = wv == 0 ? ga : ea;
+        for (int i0 = 0; i0 < VPT * kSelWaves; i0 += 64) {
+            const int v = list[i0 + lane], incl = wave_scan(v);
+            list[i0 + lane] = run + incl - v;
+            run += __shfl(incl, 63, 64);
+        }
+    }
+    __syncthreads();
+    const uint64_t lower = (1ull << lane) - 1;
+#pragma unroll
+    for (int e = 0; e < VPT; ++e) {
+        const bool valid = k.valid >> e & 1u;
+        const bool gt = valid && k.r[e] > threshold, eq = valid && k.r[e] == threshold;
+        const int g = s.gt[e * kSelWaves + wv] + __builtin_popcountll(__builtin_amdgcn_ballot_w64(gt) & lower);
+        const int q = s.eq[e * kSelWaves + wv] + __builtin_popcountll(__builtin_amdgcn_ballot_w64(eq) & lower);
+        if (gt || (eq && q < left)) {
+            const int j = j0 + e * kSelThreads + (int)threadIdx.x, i = g + min(q, left);
+            u.keep[i] = j;
+            u.out[i] = u.mass[j];
+        }
+    }
+}
+
+// What is there beside the kept keys: the rest of the rows, and units that keep all.
+// Threads `first`, first + `step` .. of the unit; true when there is nothing to select.
+__device__ inline bool select_rest(const SelectArgs& a, const Unit& u, int first, int step) {
+    if (u.kvh == 0 && first == 0) a.counts[u.n] = u.count;
+    for (int i = u.count + first; i < a.budget; i += step) u.keep[i] = -1;
+    for (int i = u.count + first; i < a.width; i += step) u.out[i] = 0.0f;
+    if (u.L > a.budget) return false;
+    for (int i = first; i < u.count; i += step) {
+        u.keep[i] = i;
+        u.out[i] = u.mass[i];
+    }
+    return true;
+}
+
+// One launch: a work-group per (kv head, sequence), its ranks in registers.
+template <int VPT>
+__global__ __launch_bounds__(kSelThreads) void select_kernel(SelectArgs a) {
+    __shared__ SelectSmem s;
+    const Unit u = unit_of(a, blockIdx.x, blockIdx.y);
+    const int tid = threadIdx.x;
+    if (select_rest(a, u, tid, kSelThreads)) return;
+    Ranks<VPT> k;
+    k.load(a, u, 0);
+    uint32_t prefix = 0;
+    int left = u.count;
+#pragma unroll
+    for (int pass = 0; pass < 3; ++pass) {
+        s.hist[2 * tid] = s.hist[2 * tid + 1] = 0;
+        __syncthreads();
+        k.histogram(s.hist, pass, prefix);
+        __syncthreads();
+        int digit;
+        find_digit(s, s.hist[kBins - 1 - 2 * tid], s.hist[kBins - 2 - 2 * tid], left, digit, left);
+        prefix |= (uint32_t)digit << kShift[pass];
+    }
+    write_kept<VPT>(a, u, s, k, 0, prefix, left, 0, 0);
+}
+
+// The sum of a per-thread number over the work-group, in every thread.
+__device__ inline int group_total(SelectSmem& s, int v) {
+    const int lane = threadIdx.x & 63, wv = threadIdx.x >> 6;
+    const int incl = wave_scan(v);
+    if (lane == 63) s.wave_sum[wv] = incl;
+    __syncthreads();
+    int total = 0;
+    for (int i = 0; i < kSelWaves; ++i) total += s.wave_sum[i];
+    __syncthreads();
+    return total;
+}
+
+// Chunks: one launch per digit and one for the output, grid (chunks, Hkv, N).
+// Launch `pass` finds digit pass - 1 from all chunks' histograms (every
+// work-group for itself) and leaves the histogram of its own chunk's digit
+// `pass`; the last launch takes from them, too, how many of the kept keys lie in
+// the chunks before its own.
+__global__ __launch_bounds__(kSelThreads) void select_chunk_kernel(SelectArgs a, int pass) {
+    __shared__ SelectSmem s;
+    const Unit u = unit_of(a, blockIdx.y, blockIdx.z);
+    const int tid = threadIdx.x, c = blockIdx.x, chunks = (u.L + kChunk - 1) / kChunk;
+    if (pass == 3) select_rest(a, u, c * kSelThreads + tid, gridDim.x * kSelThreads);
+    if (u.L <= a.budget || c >= chunks) return;   // uniform
+    constexpr int VPT = kChunk / kSelThreads;
+    Ranks<VPT> k;
+    k.load(a, u, c * kChunk);
+    const int64_t base = u.index * a.chunks;
+    uint32_t prefix = 0;
+    int left = u.count, digit = 0;
+    int before_hi = 0, before_lo = 0;   // of the bins, in the chunks before this one
+    if (pass > 0) {
+        const int p = pass - 1;
+        if (p > 0) {   // the digits above, found by the launch before
+            prefix = (uint32_t)a.found[u.index * 4 + 2 * (p - 1)];
+            left = a.found[u.index * 4 + 2 * (p - 1) + 1];
+        }
+        const uint32_t* h = a.hist[p & 1] + base * (kBins / 2) + (kBins / 2 - 1 - tid);
+        int hi = 0, lo = 0;
+        for (int i = 0; i < chunks; ++i) {
+            const uint32_t v = h[(int64_t)i * (kBins / 2)];
+            if (i == c) {
+                before_hi = hi;
+                before_lo = lo;
+            }
+            lo += (int)(v & 0xFFFFu);
+            hi += (int)(v >> 16);
+        }
+        find_digit(s, hi, lo, left, digit, left);
+        const uint32_t above = prefix;
+        prefix |= (uint32_t)digit << kShift[p];
+        if (pass < 3) {
+            if (c == 0 && tid == 0) {
+                a.found[u.index * 4 + 2 * p] = (int)prefix;
+                a.found[u.index * 4 + 2 * p + 1] = left;
+            }
+            int n = 0;
+#pragma unroll
+            for (int e = 0; e < VPT; ++e)
+                n += (k.valid >> e & 1u) && k.matches(e, p, above) && (k.r[e] >> kShift[p]) > (prefix >> kShift[p]);
+            n = group_total(s, n);
+            if (tid == 0) a.above[p][base + c] = n;
+        }
+    }
+    if (pass < 3) {
+        s.hist[2 * tid] = s.hist[2 * tid + 1] = 0;
+        __syncthreads();
+        k.histogram(s.hist, pass, prefix);
+        __syncthreads();
+        a.hist[pass & 1][(base + c) * (kBins / 2) + tid] = (uint32_t)s.hist[2 * tid] | (uint32_t)s.hist[2 * tid + 1] << 16;
         return;
     }
-    // The count-th largest rank: `prefix` holds its digits so far, `left` how many of the
-    // ranks with that prefix are kept.
-    uint32_t prefix = 0;
-    int left = count;
-    for (int shift = 24; shift >= 0; shift -= 8) {
-        if (tid < 256) hist[tid] = 0;
-        __syncthreads();
-        for (int j = tid; j < L; j += kSelThreads) {
-            const uint32_t r = rank_at(a, mass, j, L);
-            if (shift == 24 || r >> (shift + 8) == prefix >> (shift + 8)) atomicAdd(&hist[(r >> shift) & 255], 1);
-        }
-        __syncthreads();
-        if (wv == 0) {
-            // lane l holds digits 255 - 4 l .. 252 - 4 l, the largest first
-            int h[4], sum = 0;
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                h[e] = hist[255 - 4 * lane - e];
-                sum += h[e];
-            }
-            int incl = sum;
-#pragma unroll
-            for (int off = 1; off < 64; off <<= 1) {
-                const int t = __shfl_up(incl, off, 64);
-                if (lane >= off) incl += t;
-            }
-            int before = incl - sum;
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                if (before < left && before + h[e] >= left) {
-                    s_digit = 255 - 4 * lane - e;
-                    s_left = left - before;
-                }
-                before += h[e];
-            }
-        }
-        __syncthreads();
-        prefix |= (uint32_t)s_digit << shift;
-        left = s_left;
-        __syncthreads();
-    }
-    // Kept: ranks above `prefix`, and the first `left` equal to it.
-    int above = 0, equal = 0;   // of the rounds before
-    for (int j0 = 0; j0 < L; j0 += kSelThreads) {
-        const int j = j0 + tid;
-        const uint32_t r = j < L ? rank_at(a, mass, j, L) : 0u;
-        const bool gt = j < L && r > prefix, eq = j < L && r == prefix;
-        const uint64_t bg = __builtin_amdgcn_ballot_w64(gt), be = __builtin_amdgcn_ballot_w64(eq);
-        const uint64_t lower = (1ull << lane) - 1;
-        if (lane == 0) {
-            s_above[wv] = __builtin_popcountll(bg);
-            s_equal[wv] = __builtin_popcountll(be);
-        }
-        __syncthreads();
-        int ga = above, ea = equal, gsum = 0, esum = 0;
-        for (int i = 0; i < kSelWaves; ++i) {
-            if (i < wv) {
-                ga += s_above[i];
-                ea += s_equal[i];
-            }
-            gsum += s_above[i];
-            esum += s_equal[i];
-        }
-        ga += __builtin_popcountll(bg & lower);
-        ea += __builtin_popcountll(be & lower);
-        if (gt || (eq && ea < left)) {
-            const int i = ga + min(ea, left);
-            keep[i] = j;
-            out[i] = mass[j];
-        }
-        above += gsum;
-        equal += esum;
-        __syncthreads();
-    }
+    const int bin = kBins - 1 - 2 * tid;   // the thread's bins: bin (hi), bin - 1 (lo)
+    int ga = (bin > digit ? before_hi : 0) + (bin - 1 > digit ? before_lo : 0);
+    for (int i = tid; i < c; i += kSelThreads) ga += a.above[0][base + i] + a.above[1][base + i];
+    ga = group_total(s, ga);
+    const int ea = group_total(s, bin == digit ? before_hi : (bin - 1 == digit ? before_lo : 0));
+    write_kept<VPT>(a, u, s, k, c * kChunk, prefix, left, ga, ea);
 }
 
 struct CompactArgs {
@@ -167,25 +350,45 @@ __device__ inline int64_t part_at(const CompactArgs& a, const int* table, int bl
     return (page * a.bs + pos % a.bs) * a.row_bytes + h * a.part_bytes;
 }
 
-// Source and destination pages are different: a flat copy, one unit of K and of
-// V per lane.  Grid-stride over (sequence, kept position, head, unit).
+// Source and destination pages are different: a parallel copy.  Grid (blocks of
+// kept positions, heads, N); a work-group takes 256 / lanes_per_part positions
+// at a time, kCopies of them in flight per lane, K and V.
+constexpr int kCopies = 2;
+
 template <typename U>
-__global__ __launch_bounds__(256) void compact_copy_kernel(CompactArgs a) {
-    const int64_t total = (int64_t)a.N * a.M * a.H * a.units;
-    for (int64_t x = (int64_t)blockIdx.x * 256 + threadIdx.x; x < total; x += (int64_t)gridDim.x * 256) {
-        const int64_t part = x / a.units;
-        const int u = (int)(x - part * a.units);
-        const int64_t row = part / a.H;
-        const int h = (int)(part - row * a.H);
-        const int n = (int)(row / a.M), i = (int)(row - (int64_t)n * a.M);
-        if (i >= a.counts[n]) continue;
-        const int64_t s = part_at(a, a.src, a.src_blocks, n, h, a.keep[((int64_t)n * a.H + h) * a.M + i]);
-        const int64_t d = part_at(a, a.dst, a.dst_blocks, n, h, (a.start ? a.start[n] : 0) + i);
-        if (s < 0 || d < 0) continue;
-        const int64_t off = (int64_t)u * sizeof(U);
-        const U kk = *reinterpret_cast<const U*>(a.k + s + off), vv = *reinterpret_cast<const U*>(a.v + s + off);
-        *reinterpret_cast<U*>(a.k + d + off) = kk;
-        *reinterpret_cast<U*>(a.v + d + off) = vv;
+__global__ __launch_bounds__(256) void compact_copy_kernel(CompactArgs a, int lanes) {
+    const int n = blockIdx.z, h = blockIdx.y;
+    const int r = threadIdx.x / lanes, u0 = threadIdx.x - r * lanes, rows = 256 / lanes;
+    if (r >= rows) return;
+    const int count = min(a.counts[n], a.M), start = a.start ? a.start[n] : 0;
+    const int* keep = a.keep + ((int64_t)n * a.H + h) * a.M;
+    for (int i0 = blockIdx.x * rows * kCopies; i0 < count; i0 += gridDim.x * rows * kCopies) {
+        int64_t s[kCopies], d[kCopies];
+#pragma unroll
+        for (int e = 0; e < kCopies; ++e) {
+            const int i = i0 + e * rows + r;
+            s[e] = d[e] = -1;
+            if (i < count) {
+                s[e] = part_at(a, a.src, a.src_blocks, n, h, keep[i]);
+                d[e] = part_at(a, a.dst, a.dst_blocks, n, h, start + i);
+            }
+        }
+        for (int u = u0; u < a.units; u += lanes) {
+            const int64_t off = (int64_t)u * sizeof(U);
+            U kk[kCopies], vv[kCopies];
+#pragma unroll
+            for (int e = 0; e < kCopies; ++e)
+                if (s[e] >= 0 && d[e] >= 0) {
+                    kk[e] = *reinterpret_cast<const U*>(a.k + s[e] + off);
+                    vv[e] = *reinterpret_cast<const U*>(a.v + s[e] + off);
+                }
+#pragma unroll
+            for (int e = 0; e < kCopies; ++e)
+                if (s[e] >= 0 && d[e] >= 0) {
+                    *reinterpret_cast<U*>(a.k + d[e] + off) = kk[e];
+                    *reinterpret_cast<U*>(a.v + d[e] + off) = vv[e];
+                }
+        }
     }
 }
 
@@ -235,6 +438,29 @@ __global__ __launch_bounds__(256) void compact_inplace_kernel(CompactArgs a) {
     }
 }
 
+struct SelectPlan {
+    int chunks = 0;   // 0: one launch, no workspace
+    size_t hist[2], above[2], found, total = 0;
+};
+
+SelectPlan select_plan(int N, int Hkv, int max_len) {
+    SelectPlan p;
+    if (max_len <= kOnePass * kSelThreads) return p;
+    p.chunks = (int)(((int64_t)max_len + kChunk - 1) / kChunk);
+    const size_t parts = (size_t)N * Hkv * p.chunks;
+    for (int i = 0; i < 2; ++i) {
+        p.hist[i] = p.total;
+        p.total += parts * (kBins / 2) * sizeof(uint32_t);
+    }
+    for (int i = 0; i < 2; ++i) {
+        p.above[i] = p.total;
+        p.total += (parts * sizeof(int) + 15) & ~(size_t)15;
+    }
+    p.found = p.total;
+    p.total += (size_t)N * Hkv * 4 * sizeof(int);
+    return p;
+}
+
 int unit_bytes(int64_t part_bytes, const void* k, const void* v) {
     const uintptr_t m = (uintptr_t)k | (uintptr_t)v | (uintptr_t)part_bytes;
     return (m & 15) == 0 ? 16 : (m & 7) == 0 ? 8 : (m & 3) == 0 ? 4 : 2;
@@ -243,12 +469,9 @@ int unit_bytes(int64_t part_bytes, const void* k, const void* v) {
 template <typename U>
 void launch_compact(CompactArgs a, bool in_place, hipStream_t st) {
     a.units = (int)(a.part_bytes / sizeof(U));
-    if (!in_place) {
-        const int64_t total = (int64_t)a.N * a.M * a.H * a.units;
-        const unsigned grid = (unsigned)std::min<int64_t>((total + 255) / 256, 1 << 20);
-        compact_copy_kernel<U><<<grid, 256, 0, st>>>(a);
-        return;
-    }
+    int lanes = 1;   // of a part: a power of two up to the work-group
+    while (lanes < a.units && lanes < 256) lanes *= 2;
+    const int per = 256 / lanes * kCopies;
     constexpr int kMost = 32767;   // sequences per launch (a grid's extent in z)
     const int N = a.N;
     for (int n0 = 0; n0 < N; n0 += kMost) {
@@ -258,6 +481,11 @@ void launch_compact(CompactArgs a, bool in_place, hipStream_t st) {
         b.keep += (int64_t)n0 * a.H * a.M;
         b.counts += n0;
         if (b.start) b.start += n0;
+        if (!in_place) {
+            b.dst += (int64_t)n0 * a.dst_blocks;
+            compact_copy_kernel<U><<<dim3((a.M + per - 1) / per, a.H, b.N), 256, 0, st>>>(b, lanes);
+            continue;
+        }
         compact_inplace_kernel<U><<<dim3((a.units + kUnits - 1) / kUnits, a.H, 2 * b.N), 256, 0, st>>>(b);
     }
 }
@@ -267,10 +495,16 @@ void launch_compact(CompactArgs a, bool in_place, hipStream_t st) {
 
 using namespace llkv;
 
+extern "C" size_t llkv_evict_select_workspace_size(int num_seqs, int num_kv_heads, int max_seq_len) {
+    if (num_seqs <= 0 || num_kv_heads <= 0 || max_seq_len < 0 || max_seq_len > INT32_MAX - kChunk) return 0;
+    return select_plan(num_seqs, num_kv_heads, max_seq_len).total;
+}
+
 extern "C" int llkv_evict_select(int* keep, int* counts, float* mass_out, int64_t out_seq_stride,
                                  int64_t out_head_stride, int out_width, const float* mass, int64_t mass_seq_stride,
                                  int64_t mass_head_stride, const int* seq_lens, int num_seqs, int num_kv_heads,
-                                 int max_seq_len, int budget, int sinks, int recent, void* stream) {
+                                 int max_seq_len, int budget, int sinks, int recent, void* workspace,
+                                 size_t workspace_bytes, void* stream) {
     const char* fn = "llkv_evict_select";
     if (num_seqs == 0) return LLKV_OK;
     if (num_seqs < 0 || num_kv_heads <= 0 || max_seq_len < 0)
@@ -285,8 +519,12 @@ extern "C" int llkv_evict_select(int* keep, int* counts, float* mass_out, int64_
         (num_seqs > 1 && out_seq_stride < (int64_t)num_kv_heads * out_head_stride))
         return set_error(LLKV_ERR_INVALID, "%s: %d kept totals do not fit rows of %d", fn, std::min(budget, max_seq_len),
                          out_width);
-    if (max_seq_len > INT32_MAX - 2 * kSelThreads || num_seqs > 65535)
+    if (max_seq_len > INT32_MAX - kChunk || num_seqs > 65535 || num_kv_heads > 65535)
         return set_error(LLKV_ERR_UNSUPPORTED, "%s: too many sequences or keys", fn);
+    const SelectPlan p = select_plan(num_seqs, num_kv_heads, max_seq_len);
+    if (workspace_bytes < p.total || (p.total > 0 && !workspace))
+        return set_error(LLKV_ERR_WORKSPACE, "%s: workspace of %zu bytes, %zu needed", fn, workspace_bytes, p.total);
+    if (((uintptr_t)workspace & 15) != 0) return set_error(LLKV_ERR_INVALID, "%s: workspace not 16-byte aligned", fn);
     SelectArgs a = {};
     a.mass = mass;
     a.lens = seq_lens;
@@ -303,7 +541,23 @@ extern "C" int llkv_evict_select(int* keep, int* counts, float* mass_out, int64_
     a.recent = recent;
     a.max_len = max_seq_len;
     a.Hkv = num_kv_heads;
-    select_kernel<<<dim3(num_kv_heads, num_seqs), kSelThreads, 0, (hipStream_t)stream>>>(a);
+    hipStream_t st = (hipStream_t)stream;
+    const dim3 units(num_kv_heads, num_seqs);
+    if (p.chunks > 0) {
+        char* ws = reinterpret_cast<char*>(workspace);
+        a.chunks = p.chunks;
+        for (int i = 0; i < 2; ++i) {
+            a.hist[i] = reinterpret_cast<uint32_t*>(ws + p.hist[i]);
+            a.above[i] = reinterpret_cast<int*>(ws + p.above[i]);
+        }
+        a.found = reinterpret_cast<int*>(ws + p.found);
+        const dim3 grid(p.chunks, num_kv_heads, num_seqs);
+        for (int pass = 0; pass < 4; ++pass) select_chunk_kernel<<<grid, kSelThreads, 0, st>>>(a, pass);
+    } else if (max_seq_len <= 4 * kSelThreads) {
+        select_kernel<4><<<units, kSelThreads, 0, st>>>(a);
+    } else {
+        select_kernel<kOnePass><<<units, kSelThreads, 0, st>>>(a);
+    }
     return check_launch(fn);
 }
 

@@ -447,72 +447,90 @@ def first_prefill_attn_batched(out: torch.Tensor, q: torch.Tensor, k: torch.Tens
 # calls on different streams share none, and a captured call owns its own.
 # ---------------------------------------------------------------------------
 
-def _device_of(pool: torch.Tensor) -> int:
-    """The device of a call: the pool's, which has to be the current one."""
-    if not pool.is_cuda:
-        raise ValueError("the pools must be on a GPU")
-    index = pool.device.index
-    if index != torch._C._cuda_getDevice():
-        raise ValueError(f"the pools are on cuda:{index}, which is not the current device")
-    return index
+# One expression for what a call almost always finds; the reasons are looked for afterwards (a
+# one-token qk_norm_rope_append checks ten tensors: 18.1 us a call with a test per property).
+def _device_of(t: torch.Tensor, what: str = "the pools") -> int:
+    """The device of a call: the pools', which has to be the current one."""
+    device = t.get_device()
+    if device < 0:
+        raise ValueError(f"{what} must be on a GPU")
+    if device != torch._C._cuda_getDevice():
+        raise ValueError(f"{what} must be on the current device, not on cuda:{device}")
+    return device
 
 
 def _check(t: torch.Tensor, dtype: torch.dtype, shape: tuple, device: int, name: str):
-    """`t` is contiguous, of this type, on this device, with this shape (None: any extent)."""
+    """`t` is contiguous, of this type and shape, on this device."""
+    if t.dtype is dtype and t.shape == shape and t.get_device() == device and t.is_contiguous():
+        return
     _require(t, dtype, name)
-    if t.dim() != len(shape) or any(n is not None and n != m for n, m in zip(shape, t.shape)):
+    if t.shape != shape:
         raise ValueError(f"{name}: expected shape {shape}, got {tuple(t.shape)}")
-    if t.get_device() != device:
-        raise ValueError(f"{name}: must be on cuda:{device}")
+    raise ValueError(f"{name}: must be on cuda:{device}")
+
+
+def _check_table(t: torch.Tensor, n: int, device: int, name: str) -> int:
+    """An int32 table of n rows; returns their width."""
+    width = t.shape[-1] if t.dim() == 2 else None
+    _check(t, torch.int32, (n, width), device, name)
+    return width
 
 
 def _check_pools(k_pool: torch.Tensor, v_pool: Optional[torch.Tensor]):
+    """(device, type, block size, kv heads, head_dim) of the pools."""
     device = _device_of(k_pool)
-    dtype_code(k_pool.dtype)
-    _check(k_pool, k_pool.dtype, (None,) * 4, device, "k_pool")
+    dtype, shape = k_pool.dtype, k_pool.shape
+    if len(shape) != 4 or not k_pool.is_contiguous():
+        raise ValueError("k_pool: expected contiguous [pages, block size, kv heads, head_dim]")
     if v_pool is not None:
-        _check(v_pool, k_pool.dtype, tuple(k_pool.shape), device, "v_pool")
-    return device
+        _check(v_pool, dtype, shape, device, "v_pool")
+    return device, dtype, shape[1], shape[2], shape[3]
 
 
 def _check_rows(t: torch.Tensor, dtype: torch.dtype, shape: tuple, device: int, name: str) -> int:
     """Rows [T, heads, D] whose heads are contiguous; returns the elements between tokens."""
+    strides = t.stride()
+    if (t.dtype is dtype and t.shape == shape and t.get_device() == device and strides[2] == 1
+            and strides[1] == shape[2]):
+        return strides[0]
     if t.dtype != dtype:
         raise TypeError(f"{name}: expected {dtype}, got {t.dtype}")
-    if tuple(t.shape) != shape:
+    if t.shape != shape:
         raise ValueError(f"{name}: expected shape {shape}, got {tuple(t.shape)}")
-    if t.numel() and (t.stride(2) != 1 and t.shape[2] > 1 or t.stride(1) != t.shape[2] and t.shape[1] > 1):
-        raise ValueError(f"{name}: the heads of a token must be contiguous")
     if t.get_device() != device:
         raise ValueError(f"{name}: must be on cuda:{device}")
-    return t.stride(0)
+    if t.numel() and (strides[2] != 1 and shape[2] > 1 or strides[1] != shape[2] and shape[1] > 1):
+        raise ValueError(f"{name}: the heads of a token must be contiguous")
+    return strides[0]
 
 
-def _check_mass(mass: torch.Tensor, n: int, hkv: int, device: int, name: str = "mass"):
-    """Totals [N, Hkv, width] with contiguous rows of keys; returns their strides."""
+def _check_mass(mass: torch.Tensor, n: int, hkv: int, least: int, device: int):
+    """Totals [N, Hkv, at least `least` keys] with contiguous rows of keys; returns their strides."""
     if mass.dtype != torch.float32:
-        raise TypeError(f"{name}: expected torch.float32, got {mass.dtype}")
+        raise TypeError(f"mass: expected torch.float32, got {mass.dtype}")
     if mass.dim() != 3 or mass.shape[0] != n or mass.shape[1] != hkv:
-        raise ValueError(f"{name}: expected shape ({n}, {hkv}, keys), got {tuple(mass.shape)}")
+        raise ValueError(f"mass: expected shape ({n}, {hkv}, keys), got {tuple(mass.shape)}")
     if mass.get_device() != device:
-        raise ValueError(f"{name}: must be on cuda:{device}")
+        raise ValueError(f"mass: must be on cuda:{device}")
     width = mass.shape[2]
+    if width < least:
+        raise ValueError(f"mass: rows of {width} keys for up to {least}")
     bs, hs, ks = mass.stride()
     if hkv == 1:
         hs = width
     if n == 1:
         bs = hkv * hs
     if ks != 1 and width > 1 or hs < width or bs < hkv * hs:
-        raise ValueError(f"{name}: rows of keys must be contiguous and must not overlap")
+        raise ValueError("mass: rows of keys must be contiguous and must not overlap")
     return bs, hs
 
 
 def _empty(shape: tuple, dtype: torch.dtype, device: int, stream) -> torch.Tensor:
     """A tensor of the call's stream (memory that another stream still uses is not handed out)."""
     if stream is None:
-        return torch.empty(shape, dtype=dtype, device=torch.device("cuda", device))
+        return torch.empty(shape, dtype=dtype, device="cuda")      # the current device (_device_of)
     with torch.cuda.stream(stream):
-        return torch.empty(shape, dtype=dtype, device=torch.device("cuda", device))
+        return torch.empty(shape, dtype=dtype, device="cuda")
 
 
 def _scratch(nbytes: int, given: Optional[torch.Tensor], device: int, stream):
@@ -549,22 +567,18 @@ def qk_norm_rope_append(q: Optional[torch.Tensor], k: torch.Tensor, v: torch.Ten
     each rotated pair, len(inv_freq) small integers (host; not needed with one axis).  inv_freq: fp32.
     q_out: a new tensor by default; q itself rotates in place.  k_out: None writes the k rows to the
     pool only.  The k and v rows go to pool rows slot_mapping[t] (<0 skips)."""
-    device = _check_pools(k_pool, v_pool)
-    hkv, d = k_pool.shape[2], k_pool.shape[3]
-    if k.dim() != 3:
-        raise ValueError(f"k: expected 3 dims, got {k.dim()}")
-    dt, t = k_pool.dtype, k.shape[0]
+    device, dt, _, hkv, d = _check_pools(k_pool, v_pool)
+    t = k.shape[0]
     ks = _check_rows(k, dt, (t, hkv, d), device, "k")
     vs = _check_rows(v, dt, (t, hkv, d), device, "v")
     _check(slot_mapping, torch.int64, (t,), device, "slot_mapping")
-    if positions.dim() == 1:
-        positions = positions[None]
-    _check(positions, torch.int32, (None, t), device, "positions")
-    _check(inv_freq, torch.float32, (None,), device, "inv_freq")
-    for name, w in (("q_weight", q_weight), ("k_weight", k_weight)):
-        if w is not None:
-            _check(w, torch.float32, (d,), device, name)
-    axes, half = positions.shape[0], inv_freq.shape[0]
+    axes, half = positions.shape[0] if positions.dim() == 2 else 1, inv_freq.shape[0]
+    _check(positions, torch.int32, (axes, t) if positions.dim() == 2 else (t,), device, "positions")
+    _check(inv_freq, torch.float32, (half,), device, "inv_freq")
+    if q_weight is not None:
+        _check(q_weight, torch.float32, (d,), device, "q_weight")
+    if k_weight is not None:
+        _check(k_weight, torch.float32, (d,), device, "k_weight")
     if pair_axis is not None:
         if not isinstance(pair_axis, bytes):
             pair_axis = bytes(pair_axis)
@@ -574,13 +588,12 @@ def qk_norm_rope_append(q: Optional[torch.Tensor], k: torch.Tensor, v: torch.Ten
             raise ValueError(f"pair_axis: axis {max(pair_axis)} of {axes}")
     hq = qs = qos = kos = 0
     if q is not None:
-        if q.dim() != 3:
-            raise ValueError(f"q: expected 3 dims, got {q.dim()}")
-        hq = q.shape[1]
+        hq = q.shape[1] if q.dim() == 3 else 0
         qs = _check_rows(q, dt, (t, hq, d), device, "q")
         if q_out is None:
-            q_out = _empty((t, hq, d), dt, device, stream)
-        qos = _check_rows(q_out, dt, (t, hq, d), device, "q_out")
+            q_out, qos = _empty((t, hq, d), dt, device, stream), hq * d
+        else:
+            qos = _check_rows(q_out, dt, (t, hq, d), device, "q_out")
     elif q_out is not None:
         raise ValueError("q_out: there is no q")
     if k_out is not None:
@@ -597,9 +610,7 @@ def build_tree(parents: torch.Tensor, cu_q: torch.Tensor, seq_lens: torch.Tensor
     """(tree_mask int32 [total_q, words], positions int32 [total_q]) of drafted trees: parents int32
     [total_q] within each sequence's rows cu_q[n]:cu_q[n+1], anything outside [0, i) a root; the mask has
     node i itself and its ancestors, the position is the context's length plus the depth."""
-    if not parents.is_cuda:
-        raise ValueError("parents: must be on a GPU")
-    device = _device_of(parents)
+    device = _device_of(parents, "parents")
     n, total = seq_lens.shape[0], parents.shape[0]
     _check(parents, torch.int32, (total,), device, "parents")
     _check(seq_lens, torch.int32, (n,), device, "seq_lens")
@@ -608,9 +619,9 @@ def build_tree(parents: torch.Tensor, cu_q: torch.Tensor, seq_lens: torch.Tensor
         tree_mask = _empty((total, (max_q_len + 31) // 32), torch.int32, device, stream)
     if positions is None:
         positions = _empty((total,), torch.int32, device, stream)
-    _check(tree_mask, torch.int32, (total, None), device, "tree_mask")
+    words = _check_table(tree_mask, total, device, "tree_mask")
     _check(positions, torch.int32, (total,), device, "positions")
-    check(lib().llkv_build_tree(_ptr(tree_mask), tree_mask.shape[1], _ptr(positions), _ptr(parents), _ptr(cu_q),
+    check(lib().llkv_build_tree(_ptr(tree_mask), words, _ptr(positions), _ptr(parents), _ptr(cu_q),
                                 _ptr(seq_lens), n, total, max_q_len, _stream(stream)))
     return tree_mask, positions
 
@@ -632,23 +643,22 @@ def paged_tree_attention(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Te
     """Attention of drafted trees: q [total_q, Hq, D], sequence n owning rows cu_q[n]:cu_q[n+1], whose K
     and V are its last cached positions.  A row sees the whole context and the nodes j of its sequence
     whose bit is set in its row of tree_mask (int32 [total_q, words]; build_tree)."""
-    device = _check_pools(k_pool, v_pool)
-    _, bs, hkv, d = k_pool.shape
+    device, dtype, bs, hkv, d = _check_pools(k_pool, v_pool)
     tq, hq = q.shape[0], q.shape[1]
     n = seq_lens.shape[0]
-    _check(q, k_pool.dtype, (tq, hq, d), device, "q")
+    _check(q, dtype, (tq, hq, d), device, "q")
     _check(seq_lens, torch.int32, (n,), device, "seq_lens")
-    _check(block_table, torch.int32, (n, None), device, "block_table")
+    blocks = _check_table(block_table, n, device, "block_table")
     _check(cu_q, torch.int32, (n + 1,), device, "cu_q")
-    _check(tree_mask, torch.int32, (tq, None), device, "tree_mask")
+    words = _check_table(tree_mask, tq, device, "tree_mask")
     if out is None:
-        out = _empty(tuple(q.shape), q.dtype, device, stream)
-    _check(out, k_pool.dtype, tuple(q.shape), device, "out")
-    max_q_len, max_seq_len, dt = int(max_q_len), int(max_seq_len), dtype_code(q.dtype)
+        out = _empty((tq, hq, d), dtype, device, stream)
+    else:
+        _check(out, dtype, (tq, hq, d), device, "out")
+    max_q_len, max_seq_len, dt = int(max_q_len), int(max_seq_len), dtype_code(dtype)
     ws, nbytes, held = _scratch(_tree_size(n, max_q_len, hq, hkv, d, bs, max_seq_len, dt), workspace, device, stream)
     check(lib().llkv_paged_tree_attention(_ptr(out), _ptr(q), _ptr(k_pool), _ptr(v_pool), _ptr(block_table),
-                                          block_table.shape[1], _ptr(cu_q), _ptr(seq_lens), _ptr(tree_mask),
-                                          tree_mask.shape[1], n, tq, max_q_len, max_seq_len, hq, hkv, d, bs,
+                                          blocks, _ptr(cu_q), _ptr(seq_lens), _ptr(tree_mask), words, n, tq, max_q_len, max_seq_len, hq, hkv, d, bs,
                                           _scale(scale, d), dt, ws, nbytes, _stream(stream)))
     return out
 
@@ -659,23 +669,20 @@ def paged_decode_mass(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tenso
                       stream=None) -> torch.Tensor:
     """paged_decode that also adds each key's weight, summed over the query heads of its kv head, to
     mass: fp32 [B, Hkv, keys >= max_seq_len]."""
-    device = _check_pools(k_pool, v_pool)
-    _, bs, hkv, d = k_pool.shape
+    device, dtype, bs, hkv, d = _check_pools(k_pool, v_pool)
     b, hq = q.shape[0], q.shape[1]
-    _check(q, k_pool.dtype, (b, hq, d), device, "q")
+    _check(q, dtype, (b, hq, d), device, "q")
     _check(seq_lens, torch.int32, (b,), device, "seq_lens")
-    _check(block_table, torch.int32, (b, None), device, "block_table")
-    mass_bs, mass_hs = _check_mass(mass, b, hkv, device)
-    max_seq_len, dt = int(max_seq_len), dtype_code(q.dtype)
-    if mass.shape[2] < max_seq_len:
-        raise ValueError(f"mass: rows of {mass.shape[2]} keys for up to {max_seq_len}")
+    blocks = _check_table(block_table, b, device, "block_table")
+    max_seq_len, dt = int(max_seq_len), dtype_code(dtype)
+    mass_bs, mass_hs = _check_mass(mass, b, hkv, max_seq_len, device)
     if out is None:
-        out = _empty(tuple(q.shape), q.dtype, device, stream)
-    _check(out, k_pool.dtype, tuple(q.shape), device, "out")
+        out = _empty((b, hq, d), dtype, device, stream)
+    else:
+        _check(out, dtype, (b, hq, d), device, "out")
     ws, nbytes, held = _scratch(_mass_size(b, hq, hkv, d, bs, max_seq_len, dt), workspace, device, stream)
     check(lib().llkv_paged_decode_mass(_ptr(out), _ptr(mass), mass_bs, mass_hs, _ptr(q), _ptr(k_pool), _ptr(v_pool),
-                                       _ptr(block_table), _ptr(seq_lens), b, hq, hkv, d, bs, block_table.shape[1],
-                                       max_seq_len, _scale(scale, d), dt, ws, nbytes, _stream(stream)))
+                                       _ptr(block_table), _ptr(seq_lens), b, hq, hkv, d, bs, blocks, max_seq_len, _scale(scale, d), dt, ws, nbytes, _stream(stream)))
     return out
 
 
@@ -685,45 +692,39 @@ def paged_window_mass(q: torch.Tensor, k_pool: torch.Tensor, block_table: torch.
     """Adds the weights that the last rows of each sequence (q [total_q, Hq, D], rows
     cu_q[n]:cu_q[n+1] its last tokens, causal) give to each of its keys to mass, fp32 [N, Hkv,
     keys >= max_seq_len]."""
-    device = _check_pools(k_pool, None)
-    _, bs, hkv, d = k_pool.shape
+    device, dtype, bs, hkv, d = _check_pools(k_pool, None)
     tq, hq = q.shape[0], q.shape[1]
     n = seq_lens.shape[0]
-    _check(q, k_pool.dtype, (tq, hq, d), device, "q")
+    _check(q, dtype, (tq, hq, d), device, "q")
     _check(seq_lens, torch.int32, (n,), device, "seq_lens")
-    _check(block_table, torch.int32, (n, None), device, "block_table")
+    blocks = _check_table(block_table, n, device, "block_table")
     _check(cu_q, torch.int32, (n + 1,), device, "cu_q")
-    mass_bs, mass_hs = _check_mass(mass, n, hkv, device)
-    max_q_len, max_seq_len, dt = int(max_q_len), int(max_seq_len), dtype_code(q.dtype)
-    if mass.shape[2] < max_seq_len:
-        raise ValueError(f"mass: rows of {mass.shape[2]} keys for up to {max_seq_len}")
+    max_q_len, max_seq_len, dt = int(max_q_len), int(max_seq_len), dtype_code(dtype)
+    mass_bs, mass_hs = _check_mass(mass, n, hkv, max_seq_len, device)
     need = lib().llkv_paged_window_mass_workspace_size(tq, hq, max_seq_len, dt)
     ws, nbytes, held = _scratch(need, workspace, device, stream)
     check(lib().llkv_paged_window_mass(_ptr(mass), mass_bs, mass_hs, _ptr(q), _ptr(k_pool), _ptr(block_table),
-                                       block_table.shape[1], _ptr(cu_q), _ptr(seq_lens), n, tq, max_q_len,
-                                       max_seq_len, hq, hkv, d, bs, _scale(scale, d), dt, ws, nbytes,
+                                       blocks, _ptr(cu_q), _ptr(seq_lens), n, tq, max_q_len, max_seq_len, hq, hkv, d, bs, _scale(scale, d), dt, ws, nbytes,
                                        _stream(stream)))
 
 
 def evict_select(mass: torch.Tensor, seq_lens: torch.Tensor, budget: int, max_seq_len: int, sinks: int = 0,
-                 recent: int = 0, stream=None):
+                 recent: int = 0, workspace: Optional[torch.Tensor] = None, stream=None):
     """(keep int32 [N, Hkv, budget], counts int32 [N], totals like mass): for every kv head the positions to
     keep, rising, -1 behind the last: the first `sinks`, the last `recent`, and the largest totals of the rest
     (ties: the lower position); the kept totals in the same order, zeros behind them."""
-    device = _device_of(mass)
-    n, hkv = mass.shape[0], mass.shape[1]
-    mass_bs, mass_hs = _check_mass(mass, n, hkv, device)
+    device, max_seq_len = _device_of(mass, "mass"), int(max_seq_len)
+    n, hkv, width = mass.shape
+    mass_bs, mass_hs = _check_mass(mass, n, hkv, max_seq_len, device)
     _check(seq_lens, torch.int32, (n,), device, "seq_lens")
-    max_seq_len, width = int(max_seq_len), mass.shape[2]
-    if width < max_seq_len:
-        raise ValueError(f"mass: rows of {width} keys for up to {max_seq_len}")
     if budget <= 0 or sinks < 0 or recent < 0 or sinks + recent > budget:
         raise ValueError(f"a budget of {budget} for {sinks} sinks and {recent} recent keys")
     keep = _empty((n, hkv, budget), torch.int32, device, stream)
     counts = _empty((n,), torch.int32, device, stream)
     out = _empty((n, hkv, width), torch.float32, device, stream)
+    ws, nbytes, held = _scratch(lib().llkv_evict_select_workspace_size(n, hkv, max_seq_len), workspace, device, stream)
     check(lib().llkv_evict_select(_ptr(keep), _ptr(counts), _ptr(out), hkv * width, width, width, _ptr(mass), mass_bs,
-                                  mass_hs, _ptr(seq_lens), n, hkv, max_seq_len, budget, sinks, recent,
+                                  mass_hs, _ptr(seq_lens), n, hkv, max_seq_len, budget, sinks, recent, ws, nbytes,
                                   _stream(stream)))
     return keep, counts, out
 
@@ -735,22 +736,21 @@ def compact_kv(k_pool: torch.Tensor, v_pool: torch.Tensor, block_table: torch.Te
     heads alike) to positions dst_start[n] + i (0 + i): of dst_table's pages, which hold none of the rows
     read, or in place (dst_table None; keep rising, keep[i] >= dst_start + i, and pages that no other
     sequence shares)."""
-    device = _check_pools(k_pool, v_pool)
-    _, bs, hkv, d = k_pool.shape
+    device, dtype, bs, hkv, d = _check_pools(k_pool, v_pool)
     n = block_table.shape[0]
-    _check(block_table, torch.int32, (n, None), device, "block_table")
+    blocks, dst_blocks = _check_table(block_table, n, device, "block_table"), 0
     _check(counts, torch.int32, (n,), device, "counts")
-    if keep.dim() != 3 or keep.shape[1] not in (1, hkv):
+    heads, most = keep.shape[1:] if keep.dim() == 3 else (0, 0)
+    if heads != hkv and heads != 1:
         raise ValueError(f"keep: expected shape ({n}, {hkv} or 1, positions), got {tuple(keep.shape)}")
-    _check(keep, torch.int32, (n, None, None), device, "keep")
+    _check(keep, torch.int32, (n, heads, most), device, "keep")
     if dst_table is not None:
-        _check(dst_table, torch.int32, (n, None), device, "dst_table")
+        dst_blocks = _check_table(dst_table, n, device, "dst_table")
     if dst_start is not None:
         _check(dst_start, torch.int32, (n,), device, "dst_start")
-    check(lib().llkv_compact(_ptr(k_pool), _ptr(v_pool), _ptr(block_table), block_table.shape[1], _ptr(dst_table),
-                             dst_table.shape[1] if dst_table is not None else 0, _ptr(keep), keep.shape[1],
-                             keep.shape[2], _ptr(counts), _ptr(dst_start), n, hkv, d, bs, dtype_code(k_pool.dtype),
-                             _stream(stream)))
+    check(lib().llkv_compact(_ptr(k_pool), _ptr(v_pool), _ptr(block_table), blocks, _ptr(dst_table), dst_blocks,
+                             _ptr(keep), heads, most, _ptr(counts), _ptr(dst_start), n, hkv, d, bs,
+                             dtype_code(dtype), _stream(stream)))
 
 
 def evict_kv(k_pool: torch.Tensor, v_pool: torch.Tensor, block_table: torch.Tensor, seq_lens: torch.Tensor,
@@ -760,14 +760,15 @@ def evict_kv(k_pool: torch.Tensor, v_pool: torch.Tensor, block_table: torch.Tens
     their rows (compact_kv) to positions 0 .. of dst_table's pages, or of its own with dst_table None.
     Returns (keep, counts, totals): counts are the new lengths.  The rows keep the rotation of their old
     positions, and new tokens go on with theirs; the caller frees what the tables no longer need."""
-    device = _check_pools(k_pool, v_pool)
+    device, _, bs, hkv, _ = _check_pools(k_pool, v_pool)
     n = seq_lens.shape[0]
-    _check_mass(mass, n, k_pool.shape[2], device)
-    _check(block_table, torch.int32, (n, None), device, "block_table")
+    if mass.shape[:2] != (n, hkv):
+        raise ValueError(f"mass: expected shape ({n}, {hkv}, keys), got {tuple(mass.shape)}")
+    _check_table(block_table, n, device, "block_table")     # before the totals are read
     if dst_table is not None:
-        _check(dst_table, torch.int32, (n, None), device, "dst_table")
-        if dst_table.shape[1] * k_pool.shape[1] < min(budget, int(max_seq_len)):
-            raise ValueError(f"dst_table: {dst_table.shape[1]} pages for {budget} keys")
-    keep, counts, totals = evict_select(mass, seq_lens, budget, max_seq_len, sinks, recent, stream)
+        blocks = _check_table(dst_table, n, device, "dst_table")
+        if blocks * bs < min(budget, int(max_seq_len)):
+            raise ValueError(f"dst_table: {blocks} pages for {budget} keys")
+    keep, counts, totals = evict_select(mass, seq_lens, budget, max_seq_len, sinks, recent, stream=stream)
     compact_kv(k_pool, v_pool, block_table, keep, counts, dst_table, stream=stream)
     return keep, counts, totals

@@ -94,9 +94,9 @@ def test_window_mass(args, status, word):
 
 
 def select(keep=P, counts=P, out=P, out_strides=(200, 100), width=100, mass=P, strides=(200, 100), lens=P, n=2, hkv=2,
-           longest=100, budget=50, sinks=4, recent=16):
+           longest=100, budget=50, sinks=4, recent=16, ws=P, nbytes=1 << 40):
     return err(L.lib().llkv_evict_select(keep, counts, out, *out_strides, width, mass, *strides, lens, n, hkv, longest,
-                                         budget, sinks, recent, N))
+                                         budget, sinks, recent, ws, nbytes, N))
 
 
 @pytest.mark.parametrize("args,status,word", [
@@ -105,7 +105,9 @@ def select(keep=P, counts=P, out=P, out_strides=(200, 100), width=100, mass=P, s
     (dict(keep=N), 1, "null"), (dict(counts=N), 1, "null"), (dict(out=N), 1, "null"), (dict(mass=N), 1, "null"),
     (dict(lens=N), 1, "null"), (dict(strides=(200, 99)), 1, "totals"), (dict(strides=(199, 100)), 1, "totals"),
     (dict(width=49), 1, "totals"), (dict(width=101), 1, "totals"), (dict(out_strides=(199, 100)), 1, "totals"),
-    (dict(n=65536), 2, "too many"),
+    (dict(n=65536), 2, "too many"), (dict(longest=20000, strides=(40000, 20000), ws=N), 3, "workspace"),
+    (dict(longest=20000, strides=(40000, 20000), nbytes=100), 3, "workspace"),
+    (dict(ws=ctypes.c_void_p(0x1004)), 1, "aligned"),
 ], ids=str)
 def test_evict_select(args, status, word):
     rc, msg = select(**args)
