@@ -2,16 +2,19 @@
 // step that adds its attention weights to each key's total (gfx950).  The
 // schedule is in tree_attn.h.
 //
-// Body of one wave (FewCols): a page of 16 keys at a time, K and V straight
+// Bodies.  FewCols: a page of 16 keys at a time, K and V straight
 // into the operand registers of the matrix instructions in the decode's layouts
 // (decode_mfma.h), NCT tiles of 16 columns against each.  The four waves of a
 // work-group take the four pages of a tile and join their softmax states
-// through LDS at the end of a segment.
+// through LDS at the end of a segment.  ManyCols (16-bit pools, head_dim 64 / 128
+// / 256): tiles of K and V staged in LDS by direct loads, double-buffered, each
+// wave with its own 16 or 32 columns over all keys, as the prefill.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
 #include <cmath>
 
+#include "lds_dma.h"
 #include "tree_attn.h"
 
 namespace llkv {
@@ -32,6 +35,85 @@ __device__ inline uint32_t tree_bits(const int* row, int words, int j0) {
     return (uint32_t)(((uint64_t)hi << 32 | lo) >> (j0 & 31));
 }
 
+// Whether any thread of the work-group found a value of V in the tree that is not
+// finite.
+__device__ inline bool odd_segment(int& flag, bool odd) {
+    if (threadIdx.x == 0) flag = 0;
+    lds_barrier();
+    if (odd) flag = 1;
+    lds_barrier();
+    const bool any = flag != 0;
+    lds_barrier();   // before the next segment clears it
+    return any;
+}
+
+// A segment's columns with plain arithmetic, one wave per column, keys that a
+// column does not see left out: the answer where V has values that are not
+// finite among the tree's nodes.
+template <typename T, int D>
+__device__ void slow_columns(const TreeArgs& a, const TreeSeg& sg, int kcols) {
+    const int lane = threadIdx.x & 63, G = a.Hq / a.Hkv;
+    const int64_t row_elems = (int64_t)a.Hkv * D;
+    const int* bt = a.bt + (int64_t)sg.n * a.max_blocks;
+    constexpr int MD = (D + 63) / 64;
+    const int stop = min(sg.t1 * kTreeTile, sg.s.L);
+    for (int cc = threadIdx.x >> 6; cc < kcols; cc += 4) {
+        const int col = sg.c0 + cc;
+        if (col >= sg.cols) break;
+        const int node = col / G, hq = sg.kvh * G + (col - node * G);
+        const int64_t row = sg.s.q0 + node;
+        const T* q = reinterpret_cast<const T*>(a.q) + (row * a.Hq + hq) * D;
+        float m = kNegBig, l = 0.0f, acc[MD];
+#pragma unroll
+        for (int i = 0; i < MD; ++i) acc[i] = 0.0f;
+        for (int t0 = sg.t0 * kTreeTile; t0 < stop; t0 += 64) {
+            const int t = t0 + lane;
+            const bool seen = t < stop && (tree_bits(a.mask + row * a.words, a.words, t - sg.s.hist) & 1u) != 0;
+            const int64_t at = ((int64_t)max(bt[min(t, stop - 1) / kPage], 0) * kPage + t % kPage) * row_elems + sg.kvh * D;
+            float x = -INFINITY;
+            if (seen) {
+                float d0 = 0.0f, d1 = 0.0f, d2 = 0.0f, d3 = 0.0f;
+#pragma unroll 1
+                for (int d = 0; d < D; d += 4) {
+                    const T* k = reinterpret_cast<const T*>(a.k) + at + d;
+                    d0 = fmaf(Elem<T>::to_f32(q[d]), Elem<T>::to_f32(k[0]), d0);
+                    d1 = fmaf(Elem<T>::to_f32(q[d + 1]), Elem<T>::to_f32(k[1]), d1);
+                    d2 = fmaf(Elem<T>::to_f32(q[d + 2]), Elem<T>::to_f32(k[2]), d2);
+                    d3 = fmaf(Elem<T>::to_f32(q[d + 3]), Elem<T>::to_f32(k[3]), d3);
+                }
+                x = ((d0 + d1) + (d2 + d3)) * a.scale_log2;
+            }
+            const float mx = fmaxf(m, wave_max(x)), corr = fast_exp2(m - mx);
+            const float p = seen ? fast_exp2(x - mx) : 0.0f;
+            l = l * corr + wave_sum(p);
+            m = mx;
+#pragma unroll
+            for (int i = 0; i < MD; ++i) acc[i] *= corr;
+            uint64_t left = __builtin_amdgcn_ballot_w64(seen);
+            while (left != 0) {
+                const int j = __builtin_ctzll(left);
+                left &= left - 1;
+                const float pj = __shfl(p, j, 64);
+                const int64_t vj = __shfl((long long)at, j, 64);
+#pragma unroll
+                for (int i = 0; i < MD; ++i)
+                    if (lane + 64 * i < D)
+                        acc[i] = fmaf(pj, Elem<T>::to_f32(reinterpret_cast<const T*>(a.v)[vj + lane + 64 * i]), acc[i]);
+            }
+        }
+        const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+        const int64_t part = (int64_t)sg.slot * kcols + cc;
+#pragma unroll
+        for (int i = 0; i < MD; ++i) {
+            const int d = lane + 64 * i;
+            if (d >= D) break;
+            if (sg.direct) reinterpret_cast<T*>(a.out)[(row * a.Hq + hq) * D + d] = Elem<T>::from_f32(acc[i] * inv);
+            else a.part_o[part * D + d] = acc[i] * inv;
+        }
+        if (lane == 0 && !sg.direct) a.part_lse[part] = l == 0.0f ? -INFINITY : m + fast_log2(l);
+    }
+}
+
 template <typename TT, int D_, int NCT_, bool MASS>
 struct FewCols {
     using T = TT;
@@ -42,10 +124,15 @@ struct FewCols {
     static constexpr bool kF16 = Elem<T>::kDtype == LLKV_DTYPE_F16;
     using Ops = ScoreOps<T, D>;
     static constexpr int VH = (D + 63) / 64, DT = 4 * VH, MD = VH;
+    // Resident waves per SIMD that the registers are held to (the loads in flight are what
+    // bounds a few columns).
+    static constexpr int kWavesPerEU = NCT == 1 ? (D == 64 ? 4 : (D == 96 ? 3 : (D == 128 ? (k16 ? 4 : 3) : 2)))
+                                                : (NCT == 2 && D == 64 ? 3 : (NCT == 2 && D <= 128 ? 2 : 1));
 
     struct Smem {
         float acc[W][16][D];
         float ml[W][16][2];   // (max, sum)
+        int odd;
     };
 
     __device__ static void run(const TreeArgs& a, Smem& sm, const TreeSeg& sg) {
@@ -81,6 +168,7 @@ struct FewCols {
         const int npages = (L + kPage - 1) / kPage;
         const int count = sg.t1 - sg.t0;   // this wave's pages: 4 (t0 + j) + w, j < count
         int tbl = 0;
+        bool odd = false;
         for (int j = 0; j < count; ++j) {
             if ((j & 63) == 0) {   // the next 64 page ids, one per lane
                 const int pg = W * (sg.t0 + j + lane) + w;
@@ -111,31 +199,29 @@ struct FewCols {
             }
 
             // Keys that some columns do not see: the last page's rest, where V may hold
-            // anything and is taken as zero, and the tree's own, where a value that is not
-            // finite must reach the columns that see it and no other.
+            // anything and is taken as zero, and the tree's own.  A value there that is not
+            // finite must reach the columns that see it and no other, which a product with
+            // weights of zero does not give: such a segment is computed again (slow_columns).
             const int p0 = pg * kPage;
             const bool whole = p0 + kPage <= min(hist, L);   // uniform
-            bool odd = false;
             if (!whole) {
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                    const bool beyond = p0 + 4 * g + i >= L, tree = p0 + 4 * g + i >= hist;
+                    const bool beyond = p0 + 4 * g + i >= L;
+                    const bool tree = !MASS && p0 + 4 * g + i >= hist && !beyond;
 #pragma unroll
                     for (int h = 0; h < VH; ++h) {
                         if constexpr (k16) {
-                            const bool bad = !finite_bits(vh[h][i].x, kF16) || !finite_bits(vh[h][i].y, kF16);
-                            odd |= bad && tree && !beyond;
-                            if (beyond || (bad && tree)) vh[h][i] = mu32x2{0u, 0u};
+                            odd |= tree && !(finite_bits(vh[h][i].x, kF16) && finite_bits(vh[h][i].y, kF16));
+                            vh[h][i] = beyond ? mu32x2{0u, 0u} : vh[h][i];
                         } else {
-                            const bool bad = !(isfinite(vr[h][i].x) && isfinite(vr[h][i].y) && isfinite(vr[h][i].z) &&
-                                               isfinite(vr[h][i].w));
-                            odd |= bad && tree && !beyond;
-                            if (beyond || (bad && tree)) vr[h][i] = make_float4(0.f, 0.f, 0.f, 0.f);
+                            odd |= tree && !(isfinite(vr[h][i].x) && isfinite(vr[h][i].y) && isfinite(vr[h][i].z) &&
+                                             isfinite(vr[h][i].w));
+                            if (beyond) vr[h][i] = make_float4(0.f, 0.f, 0.f, 0.f);
                         }
                     }
                 }
             }
-            const bool any_odd = !whole && __builtin_amdgcn_ballot_w64(odd) != 0;
 
             mu32x2 av[VH][4];   // V^T operands of the 16-bit product
             if constexpr (k16) {
@@ -214,10 +300,15 @@ struct FewCols {
                             o[ct][4 * h + 3] = __builtin_amdgcn_mfma_f32_16x16x4f32(vr[h][i].w, p[i], o[ct][4 * h + 3], 0, 0, 0);
                         }
                 }
-                if (any_odd) add_odd(vbase + phys * kPage * row_elems, row_elems, p0, hist, L, seen, p, o[ct]);
             }
         }
 
+        if constexpr (!MASS) {
+            if (odd_segment(sm.odd, odd)) {
+                slow_columns<T, D>(a, sg, kCols);
+                return;
+            }
+        }
         // Join the waves' states, 16 columns at a time.
 #pragma unroll
         for (int ct = 0; ct < NCT; ++ct) {
@@ -274,40 +365,252 @@ struct FewCols {
         }
         lds_barrier();
     }
+};
 
-    // The products of V's values that are not finite, which the matrix instructions took as
-    // zero, added for the columns that see their keys (a masked weight of zero times infinity
-    // would be NaN).  vrow0: row 0 of the page.
-    __device__ static void add_odd(const T* vrow0, int64_t row_elems, int p0, int hist, int L, uint32_t seen,
-                                   const float (&p)[4], mf32x4 (&o)[DT]) {
-        const int lane = threadIdx.x & 63, g = lane >> 4, c = lane & 15;
-        for (int tg = 0; tg < 4; ++tg)
+// V_MFMA_F32_16X16X32 of a 16-bit type.
+template <typename T>
+__device__ inline mf32x4 mma32(const mu32x4& x, const mu32x4& y, mf32x4 c) {
+    if constexpr (Elem<T>::kDtype == LLKV_DTYPE_F16)
+        return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(mf16x8, x), __builtin_bit_cast(mf16x8, y), c, 0, 0, 0);
+    else
+        return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(mbf16x8, x), __builtin_bit_cast(mbf16x8, y), c, 0, 0, 0);
+}
+
+template <typename T>
+__device__ inline uint32_t pack_pair(float x, float y) {
+    if constexpr (Elem<T>::kDtype == LLKV_DTYPE_F16) return pack_h2(x, y);
+    else return pack_b2(x, y);
+}
+
+// K and V in LDS tiles of BN keys.  Rows are unpadded (direct loads write 1 KB
+// blocks) and their 16-byte chunks XOR-ed with the row, so that the rows that an
+// operand read takes together lie in different banks.  The key order of the K
+// operand's rows is permuted (row 8 (c / 4) + 4 h + c % 4 of a 32-key half for
+// lane c of tile h), so that a lane's scores are the 8 consecutive keys that it
+// feeds to the second product; V's operand comes by transposing LDS reads.
+template <typename TT, int D_, int NCW>
+struct ManyCols {
+    using T = TT;
+    static constexpr int D = D_, W = 4;
+    static constexpr int kCols = 16 * NCW * W;
+    static constexpr int BN = D == 256 ? 32 : 64;
+    static constexpr int KT = BN / 16, SS = BN / 32;   // key tiles, key halves of the second product
+    static constexpr int KS = D / 32, DT = D / 16;
+    static constexpr int CPR = D / 8;                  // 16-byte chunks per row
+    static constexpr int RPB = 64 / CPR;               // rows per 1 KB block
+    static constexpr int RPW = BN / W;                 // rows that a wave loads
+    static constexpr int BPW = RPW / RPB;
+    static constexpr int kWavesPerEU = 2;
+    static constexpr uint32_t kOnes = Elem<T>::kDtype == LLKV_DTYPE_F16 ? 0x3C003C00u : 0x3F803F80u;
+    static constexpr bool kF16 = Elem<T>::kDtype == LLKV_DTYPE_F16;
+
+    struct Smem {
+        alignas(16) uint16_t k[2][BN * D];
+        alignas(16) uint16_t v[2][BN * D];
+        int odd;
+    };
+
+    __device__ static int swz(int r) { return ((r & 3) | ((r >> 1) & 0xC)) & (CPR - 1); }
+    __device__ static int at(int row, int d) { return row * D + ((((d >> 3) ^ swz(row)) << 3) | (d & 7)); }
+
+    __device__ static void run(const TreeArgs& a, Smem& sm, const TreeSeg& sg) {
+        const int tid = threadIdx.x, lane = tid & 63;
+        const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
+        const int g = lane >> 4, c = lane & 15;
+        const int G = a.Hq / a.Hkv;
+        const int L = sg.s.L, hist = sg.s.hist;
+        const uint32_t row_bytes = (uint32_t)(a.Hkv * D * sizeof(T));
+        const char* kb = reinterpret_cast<const char*>(reinterpret_cast<const T*>(a.k) + (int64_t)sg.kvh * D);
+        const char* vb = reinterpret_cast<const char*>(reinterpret_cast<const T*>(a.v) + (int64_t)sg.kvh * D);
+        const int* bt = a.bt + (int64_t)sg.n * a.max_blocks;
+        const int last_page = L > 0 ? (L - 1) / kPage : 0;
+        // keys [begin, stop) in tiles of BN
+        const int begin = sg.t0 * kTreeTile;
+        const int tiles = (min(sg.t1 * kTreeTile, L) - begin + BN - 1) / BN;   // 0 or less: no key
+
+        // The wave's rows of a tile: one page or half of one.
+        uint32_t off[BPW], lds_k[2][BPW], lds_v[2][BPW];
 #pragma unroll
-            for (int ti = 0; ti < 4; ++ti) {
-                const float pt = __shfl(seen >> ti & 1u ? p[ti] : -1.0f, 16 * tg + c, 64);
-                const int pos = p0 + 4 * tg + ti;
-                if (pos < hist || pos >= L) continue;   // uniform
-                const T* vrow = vrow0 + (4 * tg + ti) * row_elems;
+        for (int j = 0; j < BPW; ++j) {
+            const int r = RPW * w + j * RPB + lane / CPR;   // row of the tile
+            off[j] = (uint32_t)(r % kPage) * row_bytes + (uint32_t)(((lane % CPR) ^ swz(r)) * 16);
 #pragma unroll
-                for (int h = 0; h < VH; ++h)
-#pragma unroll
-                    for (int i = 0; i < 4; ++i)
-#pragma unroll
-                        for (int jj = 0; jj < 4; ++jj) {
-                            const int d = 64 * h + 16 * g + 4 * i + jj;
-                            if (D % 64 != 0 && d >= D) continue;
-                            // the four dims that one lane loaded were taken as zero together
-                            bool bad = false;
-#pragma unroll
-                            for (int e = 0; e < 4; ++e) bad |= !isfinite(Elem<T>::to_f32(vrow[d - jj + e]));
-                            if (bad && pt >= 0.0f) o[4 * h + jj][i] += pt * Elem<T>::to_f32(vrow[d]);
-                        }
+            for (int b = 0; b < 2; ++b) {
+                lds_k[b][j] = lds_addr(&sm.k[b][(RPW * w + j * RPB) * D]);
+                lds_v[b][j] = lds_addr(&sm.v[b][(RPW * w + j * RPB) * D]);
             }
+        }
+        int tbl = 0;   // page ids of the wave's next 64 tiles, one per lane
+        auto load_tbl = [&](int j) {
+            tbl = bt[min((begin + (j + lane) * BN + RPW * w) / kPage, last_page)];
+        };
+        auto load_tile = [&](int j, int buf) {
+            if ((j & 63) == 0) load_tbl(j);
+            const int phys = max(__builtin_amdgcn_readlane(tbl, j & 63), 0);
+            const uint64_t base = (uint64_t)(uint32_t)phys * row_bytes * kPage;
+#pragma unroll
+            for (int i = 0; i < BPW; ++i) {
+                dma16_s(kb + base, off[i], lds_k[buf][i]);
+                dma16_s(vb + base, off[i], lds_v[buf][i]);
+            }
+        };
+        if (tiles > 0) load_tile(0, 0);
+
+        // Columns; a negative scale goes into Q's signs, so that the largest score stays the
+        // largest when scaled.
+        const float scale = fmaxf(fabsf(a.scale_log2), 1e-30f);
+        const uint32_t flip = a.scale_log2 < 0.0f ? 0x80008000u : 0u;
+        mu32x4 q[NCW][KS];
+        const int* mrow[NCW];
+        mf32x4 o[NCW][DT], osum[NCW];
+        float m[NCW];
+#pragma unroll
+        for (int nt = 0; nt < NCW; ++nt) {
+            const int col = sg.c0 + (w * NCW + nt) * 16 + c;
+            const bool valid = col < sg.cols;
+            const int node = valid ? col / G : 0;
+            const int64_t row = sg.s.q0 + node;
+            const T* qrow = reinterpret_cast<const T*>(a.q) + (row * a.Hq + sg.kvh * G + (valid ? col - node * G : 0)) * D;
+#pragma unroll
+            for (int ks = 0; ks < KS; ++ks) {
+                const mu32x4 x = *reinterpret_cast<const mu32x4*>(qrow + 32 * ks + 8 * g);
+                q[nt][ks] = valid ? x ^ flip : mu32x4{0u, 0u, 0u, 0u};
+            }
+            mrow[nt] = a.mask + row * a.words;
+#pragma unroll
+            for (int dt = 0; dt < DT; ++dt) o[nt][dt] = mf32x4{0.f, 0.f, 0.f, 0.f};
+            osum[nt] = mf32x4{0.f, 0.f, 0.f, 0.f};
+            m[nt] = kNegBig;
+        }
+        const mu32x4 ones = {kOnes, kOnes, kOnes, kOnes};
+        bool odd = false;
+
+        for (int j = 0; j < tiles; ++j) {
+            const int buf = j & 1;
+            __builtin_amdgcn_s_waitcnt(0x3F70);   // vmcnt(0): this wave's part of the tile is in LDS
+            lds_barrier();                        // everyone's; and the other buffer has been read
+            if (j + 1 < tiles) load_tile(j + 1, buf ^ 1);
+            const int key0 = begin + j * BN;
+            const bool whole = key0 + BN <= min(hist, L);   // uniform
+            if (!whole) {
+                // V beyond the last key may hold anything: zero.  Values in the tree that are not
+                // finite: the segment is computed again.
+                for (int i = tid; i < BN * CPR; i += 256) {
+                    const int r = i / CPR;
+                    mu32x4& x = *reinterpret_cast<mu32x4*>(&sm.v[buf][i * 8]);
+                    if (key0 + r >= L) x = mu32x4{0u, 0u, 0u, 0u};
+                    else if (key0 + r >= hist)
+                        odd |= !(finite_bits(x.x, kF16) && finite_bits(x.y, kF16) && finite_bits(x.z, kF16) && finite_bits(x.w, kF16));
+                }
+                lds_barrier();
+            }
+            // S^T = K Q^T
+            mf32x4 s[KT][NCW];
+#pragma unroll
+            for (int ks = 0; ks < KS; ++ks)
+#pragma unroll
+                for (int kt = 0; kt < KT; ++kt) {
+                    const int row = 32 * (kt >> 1) + 8 * (c >> 2) + 4 * (kt & 1) + (c & 3);
+                    const mu32x4 ka = *reinterpret_cast<const mu32x4*>(&sm.k[buf][at(row, ks * 32 + g * 8)]);
+#pragma unroll
+                    for (int nt = 0; nt < NCW; ++nt)
+                        s[kt][nt] = mma32<T>(ka, q[nt][ks], ks == 0 ? mf32x4{0.f, 0.f, 0.f, 0.f} : s[kt][nt]);
+                }
+            float mx[NCW];
+            bool grow = false;
+#pragma unroll
+            for (int nt = 0; nt < NCW; ++nt) {
+                if (!whole) {
+#pragma unroll
+                    for (int kt = 0; kt < KT; ++kt) {
+                        const int k4 = key0 + 32 * (kt >> 1) + 8 * g + 4 * (kt & 1);
+                        uint32_t seen = tree_bits(mrow[nt], a.words, k4 - hist);
+                        seen &= L >= k4 + 4 ? ~0u : (1u << max(L - k4, 0)) - 1u;
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) s[kt][nt][i] = seen >> i & 1u ? s[kt][nt][i] : -INFINITY;
+                    }
+                }
+                float v = -INFINITY;
+#pragma unroll
+                for (int kt = 0; kt < KT; ++kt)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) v = fmaxf(v, s[kt][nt][i]);
+                mx[nt] = v * scale;
+                grow |= mx[nt] > m[nt] + 8.0f;
+            }
+            // The running maximum moves only when a lane's keys exceed it by more than 8.
+            if (__builtin_amdgcn_ballot_w64(grow) != 0) {
+#pragma unroll
+                for (int nt = 0; nt < NCW; ++nt) {
+                    float v = fmaxf(mx[nt], __shfl_xor(mx[nt], 16, 64));
+                    v = fmaxf(v, __shfl_xor(v, 32, 64));
+                    const float mnew = fmaxf(m[nt], v);
+                    const float corr = fast_exp2(m[nt] - mnew);
+                    m[nt] = mnew;
+                    osum[nt] *= corr;
+#pragma unroll
+                    for (int dt = 0; dt < DT; ++dt) o[nt][dt] *= corr;
+                }
+            }
+            // P in the pool's type (half a step of each weight, as the prefill), its row sums by
+            // the same rounded weights; O^T += V^T P^T.
+#pragma unroll
+            for (int ss = 0; ss < SS; ++ss) {
+                mu32x4 p[NCW];
+#pragma unroll
+                for (int nt = 0; nt < NCW; ++nt) {
+                    float e[8];
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) e[i] = fast_exp2(fmaf(s[2 * ss + (i >> 2)][nt][i & 3], scale, -m[nt]));
+                    p[nt] = mu32x4{pack_pair<T>(e[0], e[1]), pack_pair<T>(e[2], e[3]), pack_pair<T>(e[4], e[5]),
+                                   pack_pair<T>(e[6], e[7])};
+                    osum[nt] = mma32<T>(ones, p[nt], osum[nt]);
+                }
+#pragma unroll
+                for (int dt = 0; dt < DT; ++dt) {
+                    typedef short s16x4 __attribute__((ext_vector_type(4)));
+                    const int r0 = 32 * ss + 8 * g + (c >> 2), d = dt * 16 + 4 * (c & 3);
+                    const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                        (__attribute__((address_space(3))) s16x4*)(&sm.v[buf][at(r0, d)]));
+                    const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                        (__attribute__((address_space(3))) s16x4*)(&sm.v[buf][at(r0 + 4, d)]));
+                    const mu32x2 l2 = __builtin_bit_cast(mu32x2, lo), h2 = __builtin_bit_cast(mu32x2, hi);
+                    const mu32x4 va = {l2.x, l2.y, h2.x, h2.y};
+#pragma unroll
+                    for (int nt = 0; nt < NCW; ++nt) o[nt][dt] = mma32<T>(va, p[nt], o[nt][dt]);
+                }
+            }
+        }
+        if (odd_segment(sm.odd, odd)) {
+            slow_columns<T, D>(a, sg, kCols);
+            return;
+        }
+#pragma unroll
+        for (int nt = 0; nt < NCW; ++nt) {
+            const int cc = (w * NCW + nt) * 16 + c, col = sg.c0 + cc;
+            if (col >= sg.cols) continue;
+            const float sum = osum[nt][0], inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+            const int node = col / G;
+            T* out = reinterpret_cast<T*>(a.out) + ((int64_t)(sg.s.q0 + node) * a.Hq + sg.kvh * G + (col - node * G)) * D;
+            const int64_t part = (int64_t)sg.slot * kCols + cc;
+#pragma unroll
+            for (int dt = 0; dt < DT; ++dt) {
+                const mf32x4 x = o[nt][dt] * inv;
+                const int d = dt * 16 + 4 * g;
+                if (sg.direct)
+                    *reinterpret_cast<mu32x2*>(out + d) = mu32x2{pack_pair<T>(x[0], x[1]), pack_pair<T>(x[2], x[3])};
+                else
+                    *reinterpret_cast<mf32x4*>(a.part_o + part * D + d) = x;
+            }
+            if (g == 0 && !sg.direct) a.part_lse[part] = sum == 0.0f ? -INFINITY : m[nt] + fast_log2(sum);
+        }
     }
 };
 
+constexpr int kXcds = 8;
+
 template <class B>
-__global__ __launch_bounds__(256) void tree_kernel(TreeArgs a) {
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(B::kWavesPerEU))) void tree_kernel(TreeArgs a) {
     __shared__ typename B::Smem sm;
     __shared__ int64_t sP[kTreeSeqs + 1];
     tree_scan<B::kCols>(a, sP);
@@ -315,8 +618,11 @@ __global__ __launch_bounds__(256) void tree_kernel(TreeArgs a) {
         for (int i = threadIdx.x; i <= a.N; i += blockDim.x) a.plan[i] = sP[i];
     const int64_t T = a.Hkv * sP[a.N];
     const int nwg = tree_shares(a, T);
-    const int w = blockIdx.x;
-    if (w >= nwg) return;
+    if ((int)blockIdx.x >= nwg) return;
+    // Work-groups go to the 8 XCDs in turn: neighbouring shares, which may read the same
+    // keys for other columns, to one XCD's L2.
+    const int xcd = blockIdx.x % kXcds;
+    const int w = xcd * (nwg / kXcds) + min(xcd, nwg % kXcds) + blockIdx.x / kXcds;
     const int64_t r0 = share_begin(w, T, nwg), r1 = share_begin(w + 1, T, nwg);
     const int G = a.Hq / a.Hkv;
     for (int64_t p = r0; p < r1;) {
@@ -607,40 +913,56 @@ __global__ __launch_bounds__(256) void build_tree_kernel(int* mask, int words, i
 // ---------------------------------------------------------------------------
 typedef void (*TreeKernel)(TreeArgs);
 
-// Most column tiles whose accumulators and queries a wave's registers hold.
-template <typename T, int D>
-constexpr int most_tiles() {
-    constexpr bool k16 = Elem<T>::kDtype != LLKV_DTYPE_F32;
-    return k16 ? (D == 256 ? 2 : 4) : (D == 64 ? 4 : (D == 256 ? 1 : 2));
+// The kernel of a shape and its columns per unit.
+struct TreeChoice {
+    TreeKernel fn = nullptr;
+    int cols = 0;
+};
+
+template <class B>
+TreeChoice choice() {
+    return TreeChoice{tree_kernel<B>, B::kCols};
 }
 
+// Columns by the most that a sequence of the call has (cols): one unit where the
+// registers allow it, since a second one reads K and V again.
 template <typename T, int D>
-TreeKernel kernel_for(int nct, bool mass) {
-    constexpr int most = most_tiles<T, D>();
-    if (mass) {
-        if (nct == 1) return tree_kernel<FewCols<T, D, 1, true>>;
-        if constexpr (most >= 2) if (nct == 2) return tree_kernel<FewCols<T, D, 2, true>>;
-        if constexpr (most >= 4) if (nct == 4) return tree_kernel<FewCols<T, D, 4, true>>;
-    } else {
-        if (nct == 1) return tree_kernel<FewCols<T, D, 1, false>>;
-        if constexpr (most >= 2) if (nct == 2) return tree_kernel<FewCols<T, D, 2, false>>;
-        if constexpr (most >= 4) if (nct == 4) return tree_kernel<FewCols<T, D, 4, false>>;
+TreeChoice choose(int64_t cols, bool mass) {
+    constexpr bool k16 = Elem<T>::kDtype != LLKV_DTYPE_F32;
+    if (mass) {   // one unit per (sequence, kv head); wider groups take the generic kernel
+        if (cols <= 16) return choice<FewCols<T, D, 1, true>>();
+        if constexpr (D <= 128 || k16)
+            if (cols <= 32) return choice<FewCols<T, D, 2, true>>();
+        return TreeChoice();
     }
-    return nullptr;
+    if (cols <= 16) return choice<FewCols<T, D, 1, false>>();
+    if constexpr (k16 && D != 96) {
+        if constexpr (D <= 128) {
+            if (cols <= 32) return choice<FewCols<T, D, 2, false>>();
+            if (cols > 64) return choice<ManyCols<T, D, 2>>();
+        }
+        return choice<ManyCols<T, D, 1>>();
+    } else if constexpr (D == 256) {
+        return choice<FewCols<T, D, 1, false>>();
+    } else {
+        if constexpr (k16 || D == 64)
+            if (cols > 32) return choice<FewCols<T, D, 4, false>>();
+        return choice<FewCols<T, D, 2, false>>();
+    }
 }
 
 template <typename T>
-TreeKernel kernel_for(int D, int nct, bool mass) {
-    if (D == 64) return kernel_for<T, 64>(nct, mass);
-    if (D == 96) return kernel_for<T, 96>(nct, mass);
-    if (D == 128) return kernel_for<T, 128>(nct, mass);
-    return kernel_for<T, 256>(nct, mass);
+TreeChoice choose(int D, int64_t cols, bool mass) {
+    if (D == 64) return choose<T, 64>(cols, mass);
+    if (D == 96) return choose<T, 96>(cols, mass);
+    if (D == 128) return choose<T, 128>(cols, mass);
+    return choose<T, 256>(cols, mass);
 }
 
-TreeKernel kernel_for(int dtype, int D, int nct, bool mass) {
-    if (dtype == LLKV_DTYPE_F32) return kernel_for<float>(D, nct, mass);
-    if (dtype == LLKV_DTYPE_F16) return kernel_for<_Float16>(D, nct, mass);
-    return kernel_for<bf16_t>(D, nct, mass);
+TreeChoice choose(int dtype, int D, int64_t cols, bool mass) {
+    if (dtype == LLKV_DTYPE_F32) return choose<float>(D, cols, mass);
+    if (dtype == LLKV_DTYPE_F16) return choose<_Float16>(D, cols, mass);
+    return choose<bf16_t>(D, cols, mass);
 }
 
 template <typename T>
@@ -661,33 +983,28 @@ void launch_join(const TreeArgs& a, int cols, bool mass, hipStream_t st) {
 
 size_t up256(size_t n) { return (n + 255) & ~(size_t)255; }
 
-// How a shape runs: on the matrix kernels (nct > 0) with nwg work-groups at most,
-// and where its workspace's parts begin.
+// How a shape runs: on the matrix kernels (fn) with nwg work-groups at most, or on
+// the generic one, and where its workspace's parts begin.
 struct TreePlan {
-    int nct = 0, cols = 0, nwg = 0;
+    TreeKernel fn = nullptr;
+    int cols = 0, nwg = 0;
     int64_t score_stride = 0;
     size_t plan = 0, lse = 0, part_lse = 0, part_o = 0, scores = 0, total = 0;
 };
 
-// The schedule does not depend on pointers: unaligned calls use the scores alone.
 TreePlan make_plan(int N, int rows_most, int Hq, int Hkv, int D, int bs, int max_len, int dtype, bool mass) {
     TreePlan p;
-    const int G = Hq / Hkv;
     const int n1 = std::min(N, kTreeSeqs);
-    if (bs == kPage && (D == 64 || D == 96 || D == 128 || D == 256)) {
-        int most = 4;
-        while (most > 1 && !kernel_for(dtype, D, most, mass)) most /= 2;
-        const int64_t cols = (int64_t)rows_most * G;
-        p.nct = cols <= 16 ? 1 : (cols <= 32 ? std::min(2, most) : most);
-        if (mass && cols > 16 * p.nct) p.nct = 0;   // a unit is one column block there
-    }
-    if (p.nct > 0) {
-        p.cols = 16 * p.nct;
-        const int64_t blocks = ((int64_t)rows_most * G + p.cols - 1) / p.cols;
+    const int64_t cols = (int64_t)rows_most * (Hq / Hkv);
+    TreeChoice c;
+    if (bs == kPage && (D == 64 || D == 96 || D == 128 || D == 256)) c = choose(dtype, D, cols, mass);
+    p.fn = c.fn;
+    if (c.fn) {
+        p.cols = c.cols;
+        const int64_t blocks = (cols + c.cols - 1) / c.cols;
         const int64_t tiles = std::max<int64_t>(1, ((int64_t)max_len + kTreeTile - 1) / kTreeTile);
         const int64_t all = (int64_t)n1 * Hkv * blocks * tiles;
-        const int res = resident_workgroups((const void*)kernel_for(dtype, D, p.nct, mass), 256);
-        p.nwg = (int)std::max<int64_t>(1, std::min<int64_t>(res, all));
+        p.nwg = (int)std::max<int64_t>(1, std::min<int64_t>(resident_workgroups((const void*)c.fn, 256), all));
         p.lse = up256((size_t)(n1 + 1) * sizeof(int64_t));
         p.part_lse = p.lse + (mass ? up256((size_t)n1 * Hq * 4) : 0);
         p.part_o = p.part_lse + up256((size_t)2 * p.nwg * p.cols * 4);
@@ -714,7 +1031,7 @@ int run_tree(const char* fn, const TreeArgs& all, int rows, int rows_most, int m
     if (((uintptr_t)workspace & 15) != 0) return set_error(LLKV_ERR_INVALID, "%s: workspace not 16-byte aligned", fn);
     char* ws = reinterpret_cast<char*>(workspace);
     const size_t es = dtype_bytes(dtype);
-    const bool tuned = p.nct > 0 && aligned16(all.q, all.k, all.v, all.out);
+    const bool tuned = p.fn != nullptr && aligned16(all.q, all.k, all.v, all.out);
     for (int n0 = 0; n0 < all.N; n0 += kTreeSeqs) {
         TreeArgs a = all;
         a.N = std::min(all.N - n0, kTreeSeqs);
@@ -748,7 +1065,7 @@ int run_tree(const char* fn, const TreeArgs& all, int rows, int rows_most, int m
         a.lse = reinterpret_cast<float*>(ws + p.lse);
         a.part_lse = reinterpret_cast<float*>(ws + p.part_lse);
         a.part_o = reinterpret_cast<float*>(ws + p.part_o);
-        kernel_for(dtype, a.D, p.nct, mass)<<<p.nwg, 256, 0, st>>>(a);
+        p.fn<<<p.nwg, 256, 0, st>>>(a);
         if (dtype == LLKV_DTYPE_F32) launch_join<float>(a, p.cols, mass, st);
         else if (dtype == LLKV_DTYPE_F16) launch_join<_Float16>(a, p.cols, mass, st);
         else launch_join<bf16_t>(a, p.cols, mass, st);
