@@ -135,6 +135,27 @@ struct FewCols {
         int odd;
     };
 
+    // Q^T operand of one column (as ScoreOps::load_q, with the load outside the choice: inside
+    // it the registers of several column tiles went through scratch memory).
+    __device__ static void load_columns(const T* qrow, bool valid, int g, float scale, typename Ops::QReg (&q)[Ops::NQ]) {
+        if constexpr (k16) {
+#pragma unroll
+            for (int ks = 0; ks < Ops::NQ; ++ks) {
+                const mu32x4 x = *reinterpret_cast<const mu32x4*>(qrow + 32 * ks + 8 * g);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) q[ks][e] = valid ? x[e] : 0u;
+            }
+        } else {
+#pragma unroll
+            for (int cc = 0; cc < D / 16; ++cc) {
+                const float4 x = *reinterpret_cast<const float4*>(qrow + 16 * cc + 4 * g);
+                const float f[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+                for (int e = 0; e < 4; ++e) q[4 * cc + e] = valid ? f[e] * scale : 0.0f;
+            }
+        }
+    }
+
     __device__ static void run(const TreeArgs& a, Smem& sm, const TreeSeg& sg) {
         const int lane = threadIdx.x & 63;
         const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -156,8 +177,8 @@ struct FewCols {
             const bool valid = col < sg.cols;
             const int node = valid ? col / G : 0;
             const int64_t row = sg.s.q0 + node;
-            Ops::load_q(reinterpret_cast<const T*>(a.q) + (row * a.Hq + sg.kvh * G + (col - node * G)) * D, valid, g,
-                        a.scale_log2, q[ct]);
+            const T* qrow = reinterpret_cast<const T*>(a.q) + (row * a.Hq + sg.kvh * G + (valid ? col - node * G : 0)) * D;
+            load_columns(qrow, valid, g, a.scale_log2, q[ct]);
             mrow[ct] = MASS ? nullptr : a.mask + row * a.words;
 #pragma unroll
             for (int dt = 0; dt < DT; ++dt) o[ct][dt] = mf32x4{0.f, 0.f, 0.f, 0.f};
@@ -181,17 +202,19 @@ struct FewCols {
             typename Ops::KReg kr[Ops::NK];
             Ops::template load_k<false>(kbase + (phys * kPage + c) * row_elems, g, kr);
             float4 vr[VH][4];
-            mu32x2 vh[VH][4];
+            uint32_t vx[VH][4], vy[VH][4];   // 16-bit V: dims 0, 1 and 2, 3 of a lane's four
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 const T* vp = vbase + (phys * kPage + 4 * g + i) * row_elems + 4 * c;
 #pragma unroll
                 for (int h = 0; h < VH; ++h) {
                     if (D % 64 != 0 && 64 * h + 4 * c >= D) {   // past the head's last dim
-                        vh[h][i] = mu32x2{0u, 0u};
+                        vx[h][i] = vy[h][i] = 0u;
                         vr[h][i] = make_float4(0.f, 0.f, 0.f, 0.f);
                     } else if constexpr (k16) {
-                        vh[h][i] = load_vec<false, mu32x2>(vp + 64 * h);
+                        const mu32x2 x = load_vec<false, mu32x2>(vp + 64 * h);
+                        vx[h][i] = x.x;
+                        vy[h][i] = x.y;
                     } else {
                         vr[h][i] = Ops::template load_v4<false>(vp + 64 * h);
                     }
@@ -212,8 +235,9 @@ struct FewCols {
 #pragma unroll
                     for (int h = 0; h < VH; ++h) {
                         if constexpr (k16) {
-                            odd |= tree && !(finite_bits(vh[h][i].x, kF16) && finite_bits(vh[h][i].y, kF16));
-                            vh[h][i] = beyond ? mu32x2{0u, 0u} : vh[h][i];
+                            odd |= tree && !(finite_bits(vx[h][i], kF16) && finite_bits(vy[h][i], kF16));
+                            vx[h][i] = beyond ? 0u : vx[h][i];
+                            vy[h][i] = beyond ? 0u : vy[h][i];
                         } else {
                             odd |= tree && !(isfinite(vr[h][i].x) && isfinite(vr[h][i].y) && isfinite(vr[h][i].z) &&
                                              isfinite(vr[h][i].w));
@@ -230,9 +254,8 @@ struct FewCols {
 #pragma unroll
                     for (int jj = 0; jj < 4; ++jj) {
                         const unsigned sel = (jj & 1) ? 0x07060302u : 0x05040100u;
-                        const int wd = jj >> 1;
-                        av[h][jj] = mu32x2{__builtin_amdgcn_perm(vh[h][1][wd], vh[h][0][wd], sel),
-                                           __builtin_amdgcn_perm(vh[h][3][wd], vh[h][2][wd], sel)};
+                        av[h][jj] = jj < 2 ? mu32x2{__builtin_amdgcn_perm(vx[h][1], vx[h][0], sel), __builtin_amdgcn_perm(vx[h][3], vx[h][2], sel)}
+                                           : mu32x2{__builtin_amdgcn_perm(vy[h][1], vy[h][0], sel), __builtin_amdgcn_perm(vy[h][3], vy[h][2], sel)};
                     }
             }
 

@@ -24,7 +24,7 @@
 namespace llkv {
 
 constexpr int kTreeTile = 64;      // keys per tile: one page per wave
-constexpr int kTreeSeqs = 1024;    // sequences per launch (their prefix sums are in LDS)
+constexpr int kTreeSeqs = 512;     // sequences per launch (their prefix sums are in LDS; 1024 cost head_dim 128 a work-group per CU)
 
 struct TreeArgs {
     void* out;
@@ -38,7 +38,6 @@ struct TreeArgs {
     int words;
     int max_blocks, N, Hq, Hkv, D, bs;
     int max_len;          // keys beyond are cut off (the caller's bound)
-    float scale_log2;
     int nwg;
     int64_t* plan;        // [N + 1] prefix sums of column blocks x tiles, from the first kernel to the second
     float* part_o;        // [2 * nwg][kCols][D]
@@ -50,6 +49,7 @@ struct TreeArgs {
     int64_t score_stride;
     float* mass;
     int64_t mass_bs, mass_hs;
+    float scale_log2;     // last: beside nwg and plan the compiler loaded the three as one vector through LDS
 };
 
 struct TreeSeq {
