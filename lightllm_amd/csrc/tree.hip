@@ -13,6 +13,7 @@
 
 #include <algorithm>
 #include <cmath>
+#include <type_traits>
 
 #include "lds_dma.h"
 #include "tree_attn.h"
@@ -119,7 +120,7 @@ struct FewCols {
     using T = TT;
     static constexpr int D = D_, NCT = NCT_, W = 4;
     static constexpr int kCols = 16 * NCT;
-    static constexpr bool kMass = MASS;
+    static constexpr bool kMass = MASS, kTeams = false;
     static constexpr bool k16 = Elem<T>::kDtype != LLKV_DTYPE_F32;
     static constexpr bool kF16 = Elem<T>::kDtype == LLKV_DTYPE_F16;
     using Ops = ScoreOps<T, D>;
@@ -411,6 +412,19 @@ __device__ inline uint32_t pack_pair(float x, float y) {
 // operand's rows is permuted (row 8 (c / 4) + 4 h + c % 4 of a 32-key half for
 // lane c of tile h), so that a lane's scores are the 8 consecutive keys that it
 // feeds to the second product; V's operand comes by transposing LDS reads.
+// Instruction order of the S^T product: the K operand reads (READS per k-step) of
+// the first two k-steps, then each k-step's products followed by the reads of the
+// k-step after next.
+template <int KS, int READS, int PRODUCTS, int I = 0>
+__device__ inline void score_schedule() {
+    if constexpr (I == 0) __builtin_amdgcn_sched_group_barrier(0x100, KS > 1 ? 2 * READS : READS, 0);
+    if constexpr (I < KS) {
+        __builtin_amdgcn_sched_group_barrier(0x008, PRODUCTS, 0);
+        if constexpr (I + 2 < KS) __builtin_amdgcn_sched_group_barrier(0x100, READS, 0);
+        score_schedule<KS, READS, PRODUCTS, I + 1>();
+    }
+}
+
 template <typename TT, int D_, int NCW>
 struct ManyCols {
     using T = TT;
@@ -424,6 +438,7 @@ struct ManyCols {
     static constexpr int RPW = BN / W;                 // rows that a wave loads
     static constexpr int BPW = RPW / RPB;
     static constexpr int kWavesPerEU = 2;
+    static constexpr bool kMass = false, kTeams = true;
     static constexpr uint32_t kOnes = Elem<T>::kDtype == LLKV_DTYPE_F16 ? 0x3C003C00u : 0x3F803F80u;
     static constexpr bool kF16 = Elem<T>::kDtype == LLKV_DTYPE_F16;
 
@@ -508,8 +523,22 @@ struct ManyCols {
         const mu32x4 ones = {kOnes, kOnes, kOnes, kOnes};
         bool odd = false;
 
-        for (int j = 0; j < tiles; ++j) {
-            const int buf = j & 1;
+        // V^T operand of output dims 16 dt .. + 15 and the 32-key half ss.
+        auto v_operand = [&](int buf, int dt, int ss) {
+            typedef short s16x4 __attribute__((ext_vector_type(4)));
+            const int r0 = 32 * ss + 8 * g + (c >> 2), d = dt * 16 + 4 * (c & 3);
+            const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                (__attribute__((address_space(3))) s16x4*)(&sm.v[buf][at(r0, d)]));
+            const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                (__attribute__((address_space(3))) s16x4*)(&sm.v[buf][at(r0 + 4, d)]));
+            const mu32x2 l2 = __builtin_bit_cast(mu32x2, lo), h2 = __builtin_bit_cast(mu32x2, hi);
+            return mu32x4{l2.x, l2.y, h2.x, h2.y};
+        };
+
+        // One tile; buf = j & 1, constant in the loop below, so that LDS addresses fold into the
+        // instructions.
+        auto tile_step = [&](int j, auto bufc) {
+            constexpr int buf = decltype(bufc)::value;
             __builtin_amdgcn_s_waitcnt(0x3F70);   // vmcnt(0): this wave's part of the tile is in LDS
             lds_barrier();                        // everyone's; and the other buffer has been read
             if (j + 1 < tiles) load_tile(j + 1, buf ^ 1);
@@ -527,18 +556,35 @@ struct ManyCols {
                 }
                 lds_barrier();
             }
-            // S^T = K Q^T
+            __builtin_amdgcn_sched_barrier(0);   // the next tile's loads are issued first
+            if constexpr (D >= 128) __builtin_amdgcn_s_setprio(1);
+            // S^T = K Q^T, the K operands of k-step ks + 1 read behind the products of ks
             mf32x4 s[KT][NCW];
+            auto k_operand = [&](int kt, int ks) {
+                const int row = 32 * (kt >> 1) + 8 * (c >> 2) + 4 * (kt & 1) + (c & 3);
+                return *reinterpret_cast<const mu32x4*>(&sm.k[buf][at(row, ks * 32 + g * 8)]);
+            };
+            mu32x4 ka[2][KT];
 #pragma unroll
-            for (int ks = 0; ks < KS; ++ks)
+            for (int kt = 0; kt < KT; ++kt) ka[0][kt] = k_operand(kt, 0);
 #pragma unroll
-                for (int kt = 0; kt < KT; ++kt) {
-                    const int row = 32 * (kt >> 1) + 8 * (c >> 2) + 4 * (kt & 1) + (c & 3);
-                    const mu32x4 ka = *reinterpret_cast<const mu32x4*>(&sm.k[buf][at(row, ks * 32 + g * 8)]);
+            for (int ks = 0; ks < KS; ++ks) {
+                if (ks + 1 < KS) {
+#pragma unroll
+                    for (int kt = 0; kt < KT; ++kt) ka[(ks + 1) & 1][kt] = k_operand(kt, ks + 1);
+                }
+#pragma unroll
+                for (int kt = 0; kt < KT; ++kt)
 #pragma unroll
                     for (int nt = 0; nt < NCW; ++nt)
-                        s[kt][nt] = mma32<T>(ka, q[nt][ks], ks == 0 ? mf32x4{0.f, 0.f, 0.f, 0.f} : s[kt][nt]);
-                }
+                        s[kt][nt] = mma32<T>(ka[ks & 1][kt], q[nt][ks], ks == 0 ? mf32x4{0.f, 0.f, 0.f, 0.f} : s[kt][nt]);
+            }
+            score_schedule<KS, KT, KT * NCW>();
+            if constexpr (D >= 128) {
+                __builtin_amdgcn_sched_barrier(0);
+                __builtin_amdgcn_s_setprio(0);
+                __builtin_amdgcn_sched_barrier(0);
+            }
             float mx[NCW];
             bool grow = false;
 #pragma unroll
@@ -576,33 +622,58 @@ struct ManyCols {
                 }
             }
             // P in the pool's type (half a step of each weight, as the prefill), its row sums by
-            // the same rounded weights; O^T += V^T P^T.
+            // the same rounded weights; O^T += V^T P^T.  The exponentials of the second 32 keys
+            // are spread between the products of the first.
+            auto weight = [&](int ss, int nt, int i) { return fast_exp2(fmaf(s[2 * ss + (i >> 2)][nt][i & 3], scale, -m[nt])); };
+            auto pack = [&](const float* e) {
+                return mu32x4{pack_pair<T>(e[0], e[1]), pack_pair<T>(e[2], e[3]), pack_pair<T>(e[4], e[5]), pack_pair<T>(e[6], e[7])};
+            };
+            mu32x4 p[NCW], va[DT];
+            float e1[NCW][8];
 #pragma unroll
-            for (int ss = 0; ss < SS; ++ss) {
-                mu32x4 p[NCW];
+            for (int nt = 0; nt < NCW; ++nt) {
+                float e[8];
 #pragma unroll
-                for (int nt = 0; nt < NCW; ++nt) {
-                    float e[8];
+                for (int i = 0; i < 8; ++i) e[i] = weight(0, nt, i);
+                p[nt] = pack(e);
+            }
 #pragma unroll
-                    for (int i = 0; i < 8; ++i) e[i] = fast_exp2(fmaf(s[2 * ss + (i >> 2)][nt][i & 3], scale, -m[nt]));
-                    p[nt] = mu32x4{pack_pair<T>(e[0], e[1]), pack_pair<T>(e[2], e[3]), pack_pair<T>(e[4], e[5]),
-                                   pack_pair<T>(e[6], e[7])};
+            for (int dt = 0; dt < DT; ++dt) va[dt] = v_operand(buf, dt, 0);
+            constexpr int kMf = (DT + 1) * NCW;   // products per half
+            if constexpr (SS == 2) __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int k = 0; k < kMf; ++k) {
+                const int dt = k / NCW, nt = k % NCW;
+                if (dt < DT) {
+                    o[nt][dt] = mma32<T>(va[dt], p[nt], o[nt][dt]);
+                    if (SS == 2 && nt == NCW - 1) va[dt] = v_operand(buf, dt, 1);
+                } else {
                     osum[nt] = mma32<T>(ones, p[nt], osum[nt]);
                 }
+                if constexpr (SS == 2) {
 #pragma unroll
-                for (int dt = 0; dt < DT; ++dt) {
-                    typedef short s16x4 __attribute__((ext_vector_type(4)));
-                    const int r0 = 32 * ss + 8 * g + (c >> 2), d = dt * 16 + 4 * (c & 3);
-                    const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-                        (__attribute__((address_space(3))) s16x4*)(&sm.v[buf][at(r0, d)]));
-                    const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-                        (__attribute__((address_space(3))) s16x4*)(&sm.v[buf][at(r0 + 4, d)]));
-                    const mu32x2 l2 = __builtin_bit_cast(mu32x2, lo), h2 = __builtin_bit_cast(mu32x2, hi);
-                    const mu32x4 va = {l2.x, l2.y, h2.x, h2.y};
-#pragma unroll
-                    for (int nt = 0; nt < NCW; ++nt) o[nt][dt] = mma32<T>(va, p[nt], o[nt][dt]);
+                    for (int e = k * 8 * NCW / kMf; e < (k + 1) * 8 * NCW / kMf; ++e) e1[e >> 3][e & 7] = weight(1, e >> 3, e & 7);
+                    __builtin_amdgcn_sched_barrier(0);
                 }
             }
+            if constexpr (SS == 2) {
+#pragma unroll
+                for (int nt = 0; nt < NCW; ++nt) p[nt] = pack(e1[nt]);
+#pragma unroll
+                for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+                    for (int nt = 0; nt < NCW; ++nt) o[nt][dt] = mma32<T>(va[dt], p[nt], o[nt][dt]);
+#pragma unroll
+                for (int nt = 0; nt < NCW; ++nt) osum[nt] = mma32<T>(ones, p[nt], osum[nt]);
+            }
+        };
+        {
+            int j = 0;
+            for (; j + 1 < tiles; j += 2) {
+                tile_step(j, std::integral_constant<int, 0>());
+                tile_step(j + 1, std::integral_constant<int, 1>());
+            }
+            if (j < tiles) tile_step(j, std::integral_constant<int, 0>());
         }
         if (odd_segment(sm.odd, odd)) {
             slow_columns<T, D>(a, sg, kCols);
@@ -636,60 +707,68 @@ template <class B>
 __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(B::kWavesPerEU))) void tree_kernel(TreeArgs a) {
     __shared__ typename B::Smem sm;
     __shared__ int64_t sP[kTreeSeqs + 1];
-    tree_scan<B::kCols>(a, sP);
-    if (blockIdx.x == 0)
+    __shared__ int64_t sT[B::kTeams ? kTreeSeqs + 1 : 1];
+    __shared__ int s_most;
+    const int most = tree_scan<B::kCols>(a, sP, B::kTeams ? sT : nullptr);
+    int team = 1;
+    const int64_t* S = sP;
+    if constexpr (B::kTeams) {
+        if (threadIdx.x == 0) s_most = most;
+        lds_barrier();
+        const int b = s_most;
+        // teams where at most a fifth of the members' work is a block that a sequence does not have
+        if (b > 1 && b <= a.nwg && 4 * b * sT[a.N] <= 5 * sP[a.N]) {
+            team = b;
+            S = sT;
+        }
+    }
+    if (B::kMass && blockIdx.x == 0)
         for (int i = threadIdx.x; i <= a.N; i += blockDim.x) a.plan[i] = sP[i];
-    const int64_t T = a.Hkv * sP[a.N];
-    const int nwg = tree_shares(a, T);
-    if ((int)blockIdx.x >= nwg) return;
-    // Work-groups go to the 8 XCDs in turn: neighbouring shares, which may read the same
-    // keys for other columns, to one XCD's L2.
+    const int64_t T = a.Hkv * S[a.N];
+    const int shares = (int)min(T, (int64_t)(a.nwg / team)), used = shares * team;
+    if ((int)blockIdx.x >= used) {
+        if (!B::kMass && threadIdx.x == 0) a.cuts[blockIdx.x] = TreeCut{};
+        return;
+    }
+    // Work-groups go to the 8 XCDs in turn: neighbours, which may read the same keys for
+    // other columns, to one XCD's L2.
     const int xcd = blockIdx.x % kXcds;
-    const int w = xcd * (nwg / kXcds) + min(xcd, nwg % kXcds) + blockIdx.x / kXcds;
-    const int64_t r0 = share_begin(w, T, nwg), r1 = share_begin(w + 1, T, nwg);
+    const int w = xcd * (used / kXcds) + min(xcd, used % kXcds) + blockIdx.x / kXcds;
+    const int share = w / team, member = w - share * team;
+    const int64_t r0 = share_begin(share, T, shares), r1 = share_begin(share + 1, T, shares);
     const int G = a.Hq / a.Hkv;
+    TreeCut cut = {};
     for (int64_t p = r0; p < r1;) {
         TreeSeg sg;
-        sg.n = tree_find(sP, a.N, a.Hkv, p);
+        sg.n = tree_find(S, a.N, a.Hkv, p);
         sg.s = tree_seq(a, sg.n);
-        const TreeUnit u = tree_unit(a, sP, sg.n, tree_tiles(sg.s), p);
+        const TreeUnit u = tree_unit(a, S, sg.n, tree_tiles(sg.s), p);
         const int64_t end = u.begin + u.tiles, stop = end < r1 ? end : r1;
         sg.kvh = u.kvh;
         sg.cols = sg.s.P * G;
-        sg.c0 = u.cb * B::kCols;
+        sg.c0 = (u.cb + member) * B::kCols;
         sg.t0 = (int)(p - u.begin);
         sg.t1 = (int)(stop - u.begin);
         sg.direct = p == u.begin && stop == end;
         sg.slot = 2 * w + (p == r0 ? 0 : 1);
-        B::run(a, sm, sg);
+        if (sg.c0 < sg.cols) {   // (uniform; a team's member may have no block of this sequence)
+            if (p == u.begin && stop < end)
+                cut = TreeCut{sg.s.q0, sg.cols, sg.c0, sg.kvh, sg.slot, (int)(wg_of(end - 1, T, shares) - share) + 1, team};
+            B::run(a, sm, sg);
+        }
         p = stop;
     }
+    if (!B::kMass && threadIdx.x == 0) a.cuts[w] = cut;
 }
 
-// The unit that begins in share w and is cut at its end, with the shares
-// w .. last that hold the rest of it; false when there is none.
-__device__ inline bool cut_unit(const TreeArgs& a, int w, TreeUnit& u, int& first_slot, int& parts) {
-    const int64_t T = a.Hkv * a.plan[a.N];
-    const int nwg = tree_shares(a, T);
-    if (w >= nwg - 1) return false;   // the last share's units end with it
-    const int64_t r0 = share_begin(w, T, nwg), r1 = share_begin(w + 1, T, nwg);
-    const int n = tree_find(a.plan, a.N, a.Hkv, r1 - 1);
-    u = tree_unit(a, a.plan, n, tree_tiles(tree_seq(a, n)), r1 - 1);
-    const int64_t end = u.begin + u.tiles;
-    if (u.begin < r0 || end <= r1) return false;
-    first_slot = 2 * w + (u.begin == r0 ? 0 : 1);
-    parts = (int)(wg_of(end - 1, T, nwg) - w) + 1;
-    return true;
-}
-
-// Slot of part j of a cut unit whose first share is w.
-__device__ inline int part_slot(int w, int first_slot, int j) { return j == 0 ? first_slot : 2 * (w + j); }
+// Slot of part j of a cut unit that begins in work-group w.
+__device__ inline int part_slot(int w, int first_slot, int step, int j) { return j == 0 ? first_slot : 2 * (w + j * step); }
 
 // Log-sum-exp join of one column's parts: a wave, lane owning dims lane + 64 i.
 // Returns the column's log2-sum-exp2.
 template <typename T, int MD>
-__device__ inline float join_parts(const TreeArgs& a, int cols, int w, int first_slot, int parts, int col, T* out) {
-    constexpr int kBatch = 8;
+__device__ inline float join_parts(const TreeArgs& a, int cols, int w, int first_slot, int step, int parts, int col, T* out) {
+    constexpr int kBatch = 4;
     const int lane = threadIdx.x & 63;
     float M = -INFINITY, sum = 0.0f, o[MD];
 #pragma unroll
@@ -699,7 +778,7 @@ __device__ inline float join_parts(const TreeArgs& a, int cols, int w, int first
 #pragma unroll
         for (int j = 0; j < kBatch; ++j) {
             const bool ok = j0 + j < parts;
-            const int64_t row = (int64_t)part_slot(w, first_slot, j0 + (ok ? j : 0)) * cols + col;
+            const int64_t row = (int64_t)part_slot(w, first_slot, step, j0 + (ok ? j : 0)) * cols + col;
             lv[j] = ok ? a.part_lse[row] : -INFINITY;
 #pragma unroll
             for (int i = 0; i < MD; ++i) pv[j][i] = a.part_o[row * a.D + min(lane + 64 * i, a.D - 1)];
@@ -728,35 +807,57 @@ __device__ inline float join_parts(const TreeArgs& a, int cols, int w, int first
     return sum == 0.0f ? -INFINITY : M + fast_log2(sum);
 }
 
-// Grid (shares, columns / 4), a wave per column.
+// Grid (shares, kJoinSlices), a wave per column at a time.
+constexpr int kJoinSlices = 16;
+
 template <typename T, int MD>
 __global__ __launch_bounds__(256) void tree_join_kernel(TreeArgs a, int cols) {
-    TreeUnit u;
-    int slot, parts;
-    if (!cut_unit(a, blockIdx.x, u, slot, parts)) return;
+    const int w = blockIdx.x;
+    const TreeCut u = a.cuts[w];
+    if (u.parts == 0) return;
     const int G = a.Hq / a.Hkv;
-    const int lc = blockIdx.y * 4 + (threadIdx.x >> 6), col = u.cb * cols + lc;
-    const TreeSeq s = tree_seq(a, u.n);
-    if (col >= s.P * G) return;
-    const int node = col / G;
-    T* out = reinterpret_cast<T*>(a.out) + ((int64_t)(s.q0 + node) * a.Hq + u.kvh * G + (col - node * G)) * a.D;
-    join_parts<T, MD>(a, cols, blockIdx.x, slot, parts, lc, out);
+    for (int c = blockIdx.y * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6); c < cols; c += 4 * kJoinSlices) {
+        const int col = u.c0 + c;
+        if (col >= u.cols) return;
+        const int node = col / G;
+        T* out = reinterpret_cast<T*>(a.out) + ((int64_t)(u.q0 + node) * a.Hq + u.kvh * G + (col - node * G)) * a.D;
+        join_parts<T, MD>(a, cols, w, u.slot, u.step, u.parts, c, out);
+    }
 }
 
-// Kept weights: grid (key blocks of kMassKeys, Hkv, N).  Each work-group takes
-// the unit's log2-sum-exp2 per query head (joining the parts of a cut unit; the
-// first key block joins its output rows as well), then adds
-// sum over the group's heads of 2^(score - lse) to its keys' totals.
+// Kept weights: grid (key blocks of kMassKeys, Hkv, N), four keys per thread.  Each
+// work-group takes the unit's log2-sum-exp2 per query head (joining the parts of
+// a cut unit; the first key block joins its output rows as well), then adds
+// sum over the group's heads of 2^(score - lse) to its keys' totals.  The first
+// heads' scores are loaded before the log-sum-exps are known.
 constexpr int kMassKeys = 1024;
-constexpr int kMassGroup = 64;   // query heads of a kv head (tree_cols' most columns)
+constexpr int kMassGroup = 64;   // query heads of a kv head, at most
+constexpr int kMassAhead = 8;    // heads whose scores are in flight
 
 template <typename T, int MD>
 __global__ __launch_bounds__(256) void mass_join_kernel(TreeArgs a, int cols) {
     __shared__ float lse[kMassGroup];
     const int n = blockIdx.z, kvh = blockIdx.y, G = a.Hq / a.Hkv;
     const TreeSeq s = tree_seq(a, n);
-    if (blockIdx.x > 0 && (int)blockIdx.x * kMassKeys >= s.L) return;
-    const int lane = threadIdx.x & 63, wv = threadIdx.x >> 6;
+    const int first = blockIdx.x * kMassKeys;
+    if (first > 0 && first >= s.L) return;
+    const int lane = threadIdx.x & 63, wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int j0 = first + 4 * (int)threadIdx.x;
+    const bool mine = j0 < s.L;
+    const float* sc = a.scores + ((int64_t)n * a.Hkv + kvh) * G * a.score_stride + j0;
+    float* mass = a.mass + n * a.mass_bs + kvh * a.mass_hs + j0;
+    mf32x4 x[kMassAhead];
+    float old[4] = {0.f, 0.f, 0.f, 0.f};
+    auto load = [&](int h0) {
+#pragma unroll
+        for (int h = 0; h < kMassAhead; ++h)
+            if (mine && h0 + h < G) x[h] = *reinterpret_cast<const mf32x4*>(sc + (h0 + h) * a.score_stride);
+    };
+    load(0);
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+        if (j0 + i < s.L) old[i] = mass[i];
+
     const int64_t T_ = a.Hkv * a.plan[a.N];
     const int nwg = tree_shares(a, T_);
     const int tiles = tree_tiles(s);
@@ -769,14 +870,14 @@ __global__ __launch_bounds__(256) void mass_join_kernel(TreeArgs a, int cols) {
         if (w == last) {
             v = a.lse[hq];
         } else if (blockIdx.x == 0) {
-            v = join_parts<T, MD>(a, cols, w, slot, last - w + 1, c, reinterpret_cast<T*>(a.out) + hq * a.D);
+            v = join_parts<T, MD>(a, cols, w, slot, 1, last - w + 1, c, reinterpret_cast<T*>(a.out) + hq * a.D);
         } else {
             float M = -INFINITY, sum = 0.0f;
             for (int j = lane; j < last - w + 1; j += 64) {
-                const float x = a.part_lse[(int64_t)part_slot(w, slot, j) * cols + c];
-                const float mb = fmaxf(M, x);
+                const float y = a.part_lse[(int64_t)part_slot(w, slot, 1, j) * cols + c];
+                const float mb = fmaxf(M, y);
                 if (mb == -INFINITY) continue;
-                sum = sum * fast_exp2(M - mb) + fast_exp2(x - mb);
+                sum = sum * fast_exp2(M - mb) + fast_exp2(y - mb);
                 M = mb;
             }
             const float top = wave_max(M);
@@ -786,14 +887,20 @@ __global__ __launch_bounds__(256) void mass_join_kernel(TreeArgs a, int cols) {
         if (lane == 0) lse[c] = v == -INFINITY ? INFINITY : v;   // no finite score: no weight
     }
     __syncthreads();
-    float* mass = a.mass + n * a.mass_bs + kvh * a.mass_hs;
-    const float* sc = a.scores + ((int64_t)n * a.Hkv + kvh) * G * a.score_stride;
-    const int stop = min(s.L, ((int)blockIdx.x + 1) * kMassKeys);
-    for (int j = blockIdx.x * kMassKeys + threadIdx.x; j < stop; j += 256) {
-        float sum = 0.0f;
-        for (int c = 0; c < G; ++c) sum += fast_exp2(sc[c * a.score_stride + j] - lse[c]);
-        mass[j] += sum;
+    float sum[4] = {0.f, 0.f, 0.f, 0.f};
+    for (int h0 = 0; h0 < G; h0 += kMassAhead) {
+        if (h0 > 0) load(h0);
+#pragma unroll
+        for (int h = 0; h < kMassAhead; ++h) {
+            if (h0 + h >= G) break;
+            const float l = lse[h0 + h];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) sum[i] += fast_exp2(x[h][i] - l);
+        }
     }
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+        if (j0 + i < s.L) mass[i] = old[i] + sum[i];
 }
 
 // Any head_dim up to 256, any page size and alignment.  Tree: one wave per
@@ -948,9 +1055,11 @@ TreeChoice choice() {
 }
 
 // Columns by the most that a sequence of the call has (cols): one unit where the
-// registers allow it, since a second one reads K and V again.
+// registers allow it, since a second one reads K and V again; units of 16 columns
+// where the call does not fill the GPU otherwise (tiles: of all (sequence, kv
+// head) pairs).
 template <typename T, int D>
-TreeChoice choose(int64_t cols, bool mass) {
+TreeChoice choose(int64_t cols, int64_t tiles, bool mass) {
     constexpr bool k16 = Elem<T>::kDtype != LLKV_DTYPE_F32;
     if (mass) {   // one unit per (sequence, kv head); wider groups take the generic kernel
         if (cols <= 16) return choice<FewCols<T, D, 1, true>>();
@@ -958,7 +1067,7 @@ TreeChoice choose(int64_t cols, bool mass) {
             if (cols <= 32) return choice<FewCols<T, D, 2, true>>();
         return TreeChoice();
     }
-    if (cols <= 16) return choice<FewCols<T, D, 1, false>>();
+    if (cols <= 16 || tiles * ((cols + 63) / 64) < device_cus() / 2) return choice<FewCols<T, D, 1, false>>();
     if constexpr (k16 && D != 96) {
         if constexpr (D <= 128) {
             if (cols <= 32) return choice<FewCols<T, D, 2, false>>();
@@ -975,17 +1084,17 @@ TreeChoice choose(int64_t cols, bool mass) {
 }
 
 template <typename T>
-TreeChoice choose(int D, int64_t cols, bool mass) {
-    if (D == 64) return choose<T, 64>(cols, mass);
-    if (D == 96) return choose<T, 96>(cols, mass);
-    if (D == 128) return choose<T, 128>(cols, mass);
-    return choose<T, 256>(cols, mass);
+TreeChoice choose(int D, int64_t cols, int64_t tiles, bool mass) {
+    if (D == 64) return choose<T, 64>(cols, tiles, mass);
+    if (D == 96) return choose<T, 96>(cols, tiles, mass);
+    if (D == 128) return choose<T, 128>(cols, tiles, mass);
+    return choose<T, 256>(cols, tiles, mass);
 }
 
-TreeChoice choose(int dtype, int D, int64_t cols, bool mass) {
-    if (dtype == LLKV_DTYPE_F32) return choose<float>(D, cols, mass);
-    if (dtype == LLKV_DTYPE_F16) return choose<_Float16>(D, cols, mass);
-    return choose<bf16_t>(D, cols, mass);
+TreeChoice choose(int dtype, int D, int64_t cols, int64_t tiles, bool mass) {
+    if (dtype == LLKV_DTYPE_F32) return choose<float>(D, cols, tiles, mass);
+    if (dtype == LLKV_DTYPE_F16) return choose<_Float16>(D, cols, tiles, mass);
+    return choose<bf16_t>(D, cols, tiles, mass);
 }
 
 template <typename T>
@@ -998,7 +1107,7 @@ void launch_join(const TreeArgs& a, int cols, bool mass, hipStream_t st) {
         else mass_join_kernel<T, 4><<<grid, 256, 0, st>>>(a, cols);
         return;
     }
-    const dim3 grid(a.nwg, cols / 4);
+    const dim3 grid(a.nwg, kJoinSlices);
     if (md == 1) tree_join_kernel<T, 1><<<grid, 256, 0, st>>>(a, cols);
     else if (md == 2) tree_join_kernel<T, 2><<<grid, 256, 0, st>>>(a, cols);
     else tree_join_kernel<T, 4><<<grid, 256, 0, st>>>(a, cols);
@@ -1019,16 +1128,17 @@ TreePlan make_plan(int N, int rows_most, int Hq, int Hkv, int D, int bs, int max
     TreePlan p;
     const int n1 = std::min(N, kTreeSeqs);
     const int64_t cols = (int64_t)rows_most * (Hq / Hkv);
+    const int64_t tiles = std::max<int64_t>(1, ((int64_t)max_len + kTreeTile - 1) / kTreeTile);
     TreeChoice c;
-    if (bs == kPage && (D == 64 || D == 96 || D == 128 || D == 256)) c = choose(dtype, D, cols, mass);
+    if (bs == kPage && (D == 64 || D == 96 || D == 128 || D == 256)) c = choose(dtype, D, cols, tiles * n1 * Hkv, mass);
     p.fn = c.fn;
     if (c.fn) {
         p.cols = c.cols;
         const int64_t blocks = (cols + c.cols - 1) / c.cols;
-        const int64_t tiles = std::max<int64_t>(1, ((int64_t)max_len + kTreeTile - 1) / kTreeTile);
         const int64_t all = (int64_t)n1 * Hkv * blocks * tiles;
         p.nwg = (int)std::max<int64_t>(1, std::min<int64_t>(resident_workgroups((const void*)c.fn, 256), all));
-        p.lse = up256((size_t)(n1 + 1) * sizeof(int64_t));
+        p.plan = up256((size_t)p.nwg * sizeof(TreeCut));
+        p.lse = p.plan + up256((size_t)(n1 + 1) * sizeof(int64_t));
         p.part_lse = p.lse + (mass ? up256((size_t)n1 * Hq * 4) : 0);
         p.part_o = p.part_lse + up256((size_t)2 * p.nwg * p.cols * 4);
         p.scores = p.part_o + up256((size_t)2 * p.nwg * p.cols * D * 4);
@@ -1084,7 +1194,8 @@ int run_tree(const char* fn, const TreeArgs& all, int rows, int rows_most, int m
             continue;
         }
         a.nwg = p.nwg;
-        a.plan = reinterpret_cast<int64_t*>(ws);
+        a.cuts = reinterpret_cast<TreeCut*>(ws);
+        a.plan = reinterpret_cast<int64_t*>(ws + p.plan);
         a.lse = reinterpret_cast<float*>(ws + p.lse);
         a.part_lse = reinterpret_cast<float*>(ws + p.part_lse);
         a.part_o = reinterpret_cast<float*>(ws + p.part_o);

@@ -16,6 +16,11 @@
 // share, a normalised fp32 row and its log2-sum-exp2 per column, which a second
 // kernel joins.  A share has at most two cut units, its first and its last, so
 // that two partial slots per work-group are enough.
+//
+// Where most sequences have as many column blocks as the widest one, B > 1, the
+// work-groups form teams of B neighbours: the teams share the tiles, and each
+// member of a team runs the same tiles for a block of its own, so that K and V
+// come from HBM once and from the XCD's L2 for the others.
 #pragma once
 
 #include "attn_common.h"
@@ -25,6 +30,12 @@ namespace llkv {
 
 constexpr int kTreeTile = 64;      // keys per tile: one page per wave
 constexpr int kTreeSeqs = 512;     // sequences per launch (their prefix sums are in LDS; 1024 cost head_dim 128 a work-group per CU)
+
+// A cut unit, left by the work-group w that it begins in for the second kernel: part
+// j's slot is `slot` for j = 0, else 2 * (w + j * step).  parts 0: none begins there.
+struct TreeCut {
+    int q0, cols, c0, kvh, slot, parts, step;
+};
 
 struct TreeArgs {
     void* out;
@@ -39,7 +50,8 @@ struct TreeArgs {
     int max_blocks, N, Hq, Hkv, D, bs;
     int max_len;          // keys beyond are cut off (the caller's bound)
     int nwg;
-    int64_t* plan;        // [N + 1] prefix sums of column blocks x tiles, from the first kernel to the second
+    TreeCut* cuts;        // [nwg]
+    int64_t* plan;        // [N + 1] prefix sums of column blocks x tiles (kept weights alone)
     float* part_o;        // [2 * nwg][kCols][D]
     float* part_lse;      // [2 * nwg][kCols]
     // Kept weights: scaled scores [N * Hkv * G][score_stride], log2-sum-exp2 of
@@ -98,26 +110,45 @@ __device__ inline int64_t wave_incl_scan64(int64_t v) {
     return v;
 }
 
-// sP[n] = column blocks x tiles of sequences [0, n), n = 0 .. N; wave 0, ends with a barrier.
+// sP[n] = column blocks x tiles of sequences [0, n), n = 0 .. N, and, where sT is
+// given, sT[n] = their tiles; wave 0, ends with a barrier.  Returns the most blocks
+// of a sequence to wave 0.
 template <int COLS>
-__device__ inline void tree_scan(const TreeArgs& a, int64_t* sP) {
+__device__ inline int tree_scan(const TreeArgs& a, int64_t* sP, int64_t* sT) {
+    int most = 0;
     if (threadIdx.x < 64) {
         const int lane = threadIdx.x, G = a.Hq / a.Hkv;
-        int64_t run = 0;
+        int64_t run = 0, run_t = 0;
         for (int n0 = 0; n0 < a.N; n0 += 64) {
             const int n = n0 + lane;
-            int64_t v = 0;
+            int64_t t = 0, v = 0;
             if (n < a.N) {
                 const TreeSeq s = tree_seq(a, n);
-                v = (int64_t)tree_blocks<COLS>(s, G) * tree_tiles(s);
+                const int b = tree_blocks<COLS>(s, G);
+                t = tree_tiles(s);
+                v = b * t;
+                most = max(most, b);
             }
             const int64_t incl = wave_incl_scan64(v);
             if (n < a.N) sP[n + 1] = run + incl;
             run += __shfl((long long)incl, 63, 64);
+            if (sT) {
+                const int64_t incl_t = wave_incl_scan64(t);
+                if (n < a.N) sT[n + 1] = run_t + incl_t;
+                run_t += __shfl((long long)incl_t, 63, 64);
+            }
         }
-        if (lane == 0) sP[0] = 0;
+        if (lane == 0) {
+            sP[0] = 0;
+            if (sT) sT[0] = 0;
+        }
+        if (sT) {
+#pragma unroll
+            for (int off = 1; off < 64; off <<= 1) most = max(most, __shfl_xor(most, off, 64));
+        }
     }
     __syncthreads();
+    return most;
 }
 
 // The sequence whose tiles hold position p: Hkv * P[n] <= p < Hkv * P[n + 1].
