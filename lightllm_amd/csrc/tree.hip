@@ -58,7 +58,7 @@ __device__ void slow_columns(const TreeArgs& a, const TreeSeg& sg, int kcols) {
     const int* bt = a.bt + (int64_t)sg.n * a.max_blocks;
     constexpr int MD = (D + 63) / 64;
     const int stop = min(sg.t1 * kTreeTile, sg.s.L);
-    for (int cc = threadIdx.x >> 6; cc < kcols; cc += 4) {
+    for (int cc = threadIdx.x >> 6; cc < kcols; cc += blockDim.x >> 6) {
         const int col = sg.c0 + cc;
         if (col >= sg.cols) break;
         const int node = col / G, hq = sg.kvh * G + (col - node * G);
@@ -119,7 +119,7 @@ template <typename TT, int D_, int NCT_, bool MASS>
 struct FewCols {
     using T = TT;
     static constexpr int D = D_, NCT = NCT_, W = 4;
-    static constexpr int kCols = 16 * NCT;
+    static constexpr int kCols = 16 * NCT, kThreads = 64 * W;
     static constexpr bool kMass = MASS, kTeams = false;
     static constexpr bool k16 = Elem<T>::kDtype != LLKV_DTYPE_F32;
     static constexpr bool kF16 = Elem<T>::kDtype == LLKV_DTYPE_F16;
@@ -391,6 +391,9 @@ struct FewCols {
     }
 };
 
+// S_WAITCNT's operand for at most n vector memory operations left, the other counters free.
+constexpr int vmcnt_imm(int n) { return 0x3F70 | (n & 15) | (n >> 4) << 14; }
+
 // V_MFMA_F32_16X16X32 of a 16-bit type.
 template <typename T>
 __device__ inline mf32x4 mma32(const mu32x4& x, const mu32x4& y, mf32x4 c) {
@@ -425,11 +428,11 @@ __device__ inline void score_schedule() {
     }
 }
 
-template <typename TT, int D_, int NCW>
+template <typename TT, int D_, int NCW, int WV, int RING>
 struct ManyCols {
     using T = TT;
-    static constexpr int D = D_, W = 4;
-    static constexpr int kCols = 16 * NCW * W;
+    static constexpr int D = D_, W = WV, R = RING;
+    static constexpr int kCols = 16 * NCW * W, kThreads = 64 * W;
     static constexpr int BN = D == 256 ? 32 : 64;
     static constexpr int KT = BN / 16, SS = BN / 32;   // key tiles, key halves of the second product
     static constexpr int KS = D / 32, DT = D / 16;
@@ -443,8 +446,8 @@ struct ManyCols {
     static constexpr bool kF16 = Elem<T>::kDtype == LLKV_DTYPE_F16;
 
     struct Smem {
-        alignas(16) uint16_t k[2][BN * D];
-        alignas(16) uint16_t v[2][BN * D];
+        alignas(16) uint16_t k[R][BN * D];
+        alignas(16) uint16_t v[R][BN * D];
         int odd;
     };
 
@@ -466,33 +469,39 @@ struct ManyCols {
         const int begin = sg.t0 * kTreeTile;
         const int tiles = (min(sg.t1 * kTreeTile, L) - begin + BN - 1) / BN;   // 0 or less: no key
 
-        // The wave's rows of a tile: one page or half of one.
-        uint32_t off[BPW], lds_k[2][BPW], lds_v[2][BPW];
+        // The wave's rows of a tile: one page or a part of one.
+        constexpr uint32_t kTileBytes = BN * D * 2;
+        uint32_t off[BPW], lds_k[BPW], lds_v[BPW];
 #pragma unroll
         for (int j = 0; j < BPW; ++j) {
             const int r = RPW * w + j * RPB + lane / CPR;   // row of the tile
             off[j] = (uint32_t)(r % kPage) * row_bytes + (uint32_t)(((lane % CPR) ^ swz(r)) * 16);
-#pragma unroll
-            for (int b = 0; b < 2; ++b) {
-                lds_k[b][j] = lds_addr(&sm.k[b][(RPW * w + j * RPB) * D]);
-                lds_v[b][j] = lds_addr(&sm.v[b][(RPW * w + j * RPB) * D]);
-            }
+            lds_k[j] = lds_addr(&sm.k[0][(RPW * w + j * RPB) * D]);
+            lds_v[j] = lds_addr(&sm.v[0][(RPW * w + j * RPB) * D]);
         }
         int tbl = 0;   // page ids of the wave's next 64 tiles, one per lane
-        auto load_tbl = [&](int j) {
-            tbl = bt[min((begin + (j + lane) * BN + RPW * w) / kPage, last_page)];
-        };
-        auto load_tile = [&](int j, int buf) {
-            if ((j & 63) == 0) load_tbl(j);
+        auto load_tile = [&](int j) {
+            if ((j & 63) == 0) tbl = bt[min((begin + (j + lane) * BN + RPW * w) / kPage, last_page)];
             const int phys = max(__builtin_amdgcn_readlane(tbl, j & 63), 0);
             const uint64_t base = (uint64_t)(uint32_t)phys * row_bytes * kPage;
+            const uint32_t to = (uint32_t)(j % R) * kTileBytes;
 #pragma unroll
             for (int i = 0; i < BPW; ++i) {
-                dma16_s(kb + base, off[i], lds_k[buf][i]);
-                dma16_s(vb + base, off[i], lds_v[buf][i]);
+                dma16_s(kb + base, off[i], lds_k[i] + to);
+                dma16_s(vb + base, off[i], lds_v[i] + to);
             }
         };
-        if (tiles > 0) load_tile(0, 0);
+#pragma unroll
+        for (int j = 0; j < R - 1; ++j)
+            if (j < tiles) load_tile(j);
+
+        // Where the lane's operands lie in a tile (halves): K row 8 (c / 4) + c % 4 for each
+        // k-step, V row 8 g + c / 4 for each output tile.
+        int koff[KS], voff[DT];
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks) koff[ks] = at(8 * (c >> 2) + (c & 3), ks * 32 + g * 8);
+#pragma unroll
+        for (int dt = 0; dt < DT; ++dt) voff[dt] = at(8 * g + (c >> 2), dt * 16 + 4 * (c & 3));
 
         // Columns; a negative scale goes into Q's signs, so that the largest score stays the
         // largest when scaled.
@@ -523,33 +532,34 @@ struct ManyCols {
         const mu32x4 ones = {kOnes, kOnes, kOnes, kOnes};
         bool odd = false;
 
-        // V^T operand of output dims 16 dt .. + 15 and the 32-key half ss.
-        auto v_operand = [&](int buf, int dt, int ss) {
-            typedef short s16x4 __attribute__((ext_vector_type(4)));
-            const int r0 = 32 * ss + 8 * g + (c >> 2), d = dt * 16 + 4 * (c & 3);
-            const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-                (__attribute__((address_space(3))) s16x4*)(&sm.v[buf][at(r0, d)]));
-            const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-                (__attribute__((address_space(3))) s16x4*)(&sm.v[buf][at(r0 + 4, d)]));
-            const mu32x2 l2 = __builtin_bit_cast(mu32x2, lo), h2 = __builtin_bit_cast(mu32x2, hi);
-            return mu32x4{l2.x, l2.y, h2.x, h2.y};
-        };
-
-        // One tile; buf = j & 1, constant in the loop below, so that LDS addresses fold into the
-        // instructions.
-        auto tile_step = [&](int j, auto bufc) {
-            constexpr int buf = decltype(bufc)::value;
-            __builtin_amdgcn_s_waitcnt(0x3F70);   // vmcnt(0): this wave's part of the tile is in LDS
-            lds_barrier();                        // everyone's; and the other buffer has been read
-            if (j + 1 < tiles) load_tile(j + 1, buf ^ 1);
+        for (int j = 0; j < tiles; ++j) {
+            // This wave's part of tile j is in LDS: all loads but those of the tiles after it.
+            const int after = tiles - 1 - j;
+            constexpr int kAll = vmcnt_imm(2 * BPW * (R - 2)), kLess = vmcnt_imm(R > 2 ? 2 * BPW * (R - 3) : 0);
+            if (after >= R - 2) __builtin_amdgcn_s_waitcnt(kAll);
+            else if (after == R - 3) __builtin_amdgcn_s_waitcnt(kLess);
+            else __builtin_amdgcn_s_waitcnt(vmcnt_imm(0));
+            lds_barrier();   // everyone's; and the buffer of tile j - 1 has been read
+            if (j + R - 1 < tiles) load_tile(j + R - 1);
+            uint16_t* const kt_lds = sm.k[j % R];
+            uint16_t* const vt_lds = sm.v[j % R];
+            // V^T operand of output dims 16 dt .. + 15 and the 32-key half ss.
+            auto v_operand = [&](int dt, int ss) {
+                typedef short s16x4 __attribute__((ext_vector_type(4)));
+                const uint16_t* at0 = vt_lds + voff[dt] + 32 * ss * D;
+                const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)at0);
+                const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(at0 + 4 * D));
+                const mu32x2 l2 = __builtin_bit_cast(mu32x2, lo), h2 = __builtin_bit_cast(mu32x2, hi);
+                return mu32x4{l2.x, l2.y, h2.x, h2.y};
+            };
             const int key0 = begin + j * BN;
             const bool whole = key0 + BN <= min(hist, L);   // uniform
             if (!whole) {
                 // V beyond the last key may hold anything: zero.  Values in the tree that are not
                 // finite: the segment is computed again.
-                for (int i = tid; i < BN * CPR; i += 256) {
+                for (int i = tid; i < BN * CPR; i += kThreads) {
                     const int r = i / CPR;
-                    mu32x4& x = *reinterpret_cast<mu32x4*>(&sm.v[buf][i * 8]);
+                    mu32x4& x = *reinterpret_cast<mu32x4*>(vt_lds + i * 8);
                     if (key0 + r >= L) x = mu32x4{0u, 0u, 0u, 0u};
                     else if (key0 + r >= hist)
                         odd |= !(finite_bits(x.x, kF16) && finite_bits(x.y, kF16) && finite_bits(x.z, kF16) && finite_bits(x.w, kF16));
@@ -561,8 +571,7 @@ struct ManyCols {
             // S^T = K Q^T, the K operands of k-step ks + 1 read behind the products of ks
             mf32x4 s[KT][NCW];
             auto k_operand = [&](int kt, int ks) {
-                const int row = 32 * (kt >> 1) + 8 * (c >> 2) + 4 * (kt & 1) + (c & 3);
-                return *reinterpret_cast<const mu32x4*>(&sm.k[buf][at(row, ks * 32 + g * 8)]);
+                return *reinterpret_cast<const mu32x4*>(kt_lds + koff[ks] + (32 * (kt >> 1) + 4 * (kt & 1)) * D);
             };
             mu32x4 ka[2][KT];
 #pragma unroll
@@ -638,7 +647,7 @@ struct ManyCols {
                 p[nt] = pack(e);
             }
 #pragma unroll
-            for (int dt = 0; dt < DT; ++dt) va[dt] = v_operand(buf, dt, 0);
+            for (int dt = 0; dt < DT; ++dt) va[dt] = v_operand(dt, 0);
             constexpr int kMf = (DT + 1) * NCW;   // products per half
             if constexpr (SS == 2) __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
@@ -646,7 +655,7 @@ struct ManyCols {
                 const int dt = k / NCW, nt = k % NCW;
                 if (dt < DT) {
                     o[nt][dt] = mma32<T>(va[dt], p[nt], o[nt][dt]);
-                    if (SS == 2 && nt == NCW - 1) va[dt] = v_operand(buf, dt, 1);
+                    if (SS == 2 && nt == NCW - 1) va[dt] = v_operand(dt, 1);
                 } else {
                     osum[nt] = mma32<T>(ones, p[nt], osum[nt]);
                 }
@@ -666,14 +675,6 @@ struct ManyCols {
 #pragma unroll
                 for (int nt = 0; nt < NCW; ++nt) osum[nt] = mma32<T>(ones, p[nt], osum[nt]);
             }
-        };
-        {
-            int j = 0;
-            for (; j + 1 < tiles; j += 2) {
-                tile_step(j, std::integral_constant<int, 0>());
-                tile_step(j + 1, std::integral_constant<int, 1>());
-            }
-            if (j < tiles) tile_step(j, std::integral_constant<int, 0>());
         }
         if (odd_segment(sm.odd, odd)) {
             slow_columns<T, D>(a, sg, kCols);
@@ -704,7 +705,7 @@ struct ManyCols {
 constexpr int kXcds = 8;
 
 template <class B>
-__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(B::kWavesPerEU))) void tree_kernel(TreeArgs a) {
+__global__ __launch_bounds__(B::kThreads) __attribute__((amdgpu_waves_per_eu(B::kWavesPerEU))) void tree_kernel(TreeArgs a) {
     __shared__ typename B::Smem sm;
     __shared__ int64_t sP[kTreeSeqs + 1];
     __shared__ int64_t sT[B::kTeams ? kTreeSeqs + 1 : 1];
@@ -1046,12 +1047,12 @@ typedef void (*TreeKernel)(TreeArgs);
 // The kernel of a shape and its columns per unit.
 struct TreeChoice {
     TreeKernel fn = nullptr;
-    int cols = 0;
+    int cols = 0, threads = 0;
 };
 
 template <class B>
 TreeChoice choice() {
-    return TreeChoice{tree_kernel<B>, B::kCols};
+    return TreeChoice{tree_kernel<B>, B::kCols, B::kThreads};
 }
 
 // Columns by the most that a sequence of the call has (cols): one unit where the
@@ -1071,9 +1072,10 @@ TreeChoice choose(int64_t cols, int64_t tiles, bool mass) {
     if constexpr (k16 && D != 96) {
         if constexpr (D <= 128) {
             if (cols <= 32) return choice<FewCols<T, D, 2, false>>();
-            if (cols > 64) return choice<ManyCols<T, D, 2>>();
+            if (cols > 128) return choice<ManyCols<T, D, 2, 8, 4>>();
+            if (cols > 64) return choice<ManyCols<T, D, 2, 4, 2>>();
         }
-        return choice<ManyCols<T, D, 1>>();
+        return choice<ManyCols<T, D, 1, 4, 2>>();
     } else if constexpr (D == 256) {
         return choice<FewCols<T, D, 1, false>>();
     } else {
@@ -1119,7 +1121,7 @@ size_t up256(size_t n) { return (n + 255) & ~(size_t)255; }
 // the generic one, and where its workspace's parts begin.
 struct TreePlan {
     TreeKernel fn = nullptr;
-    int cols = 0, nwg = 0;
+    int cols = 0, threads = 0, nwg = 0;
     int64_t score_stride = 0;
     size_t plan = 0, lse = 0, part_lse = 0, part_o = 0, scores = 0, total = 0;
 };
@@ -1134,9 +1136,10 @@ TreePlan make_plan(int N, int rows_most, int Hq, int Hkv, int D, int bs, int max
     p.fn = c.fn;
     if (c.fn) {
         p.cols = c.cols;
+        p.threads = c.threads;
         const int64_t blocks = (cols + c.cols - 1) / c.cols;
         const int64_t all = (int64_t)n1 * Hkv * blocks * tiles;
-        p.nwg = (int)std::max<int64_t>(1, std::min<int64_t>(resident_workgroups((const void*)c.fn, 256), all));
+        p.nwg = (int)std::max<int64_t>(1, std::min<int64_t>(resident_workgroups((const void*)c.fn, c.threads), all));
         p.plan = up256((size_t)p.nwg * sizeof(TreeCut));
         p.lse = p.plan + up256((size_t)(n1 + 1) * sizeof(int64_t));
         p.part_lse = p.lse + (mass ? up256((size_t)n1 * Hq * 4) : 0);
@@ -1199,7 +1202,7 @@ int run_tree(const char* fn, const TreeArgs& all, int rows, int rows_most, int m
         a.lse = reinterpret_cast<float*>(ws + p.lse);
         a.part_lse = reinterpret_cast<float*>(ws + p.part_lse);
         a.part_o = reinterpret_cast<float*>(ws + p.part_o);
-        p.fn<<<p.nwg, 256, 0, st>>>(a);
+        p.fn<<<p.nwg, p.threads, 0, st>>>(a);
         if (dtype == LLKV_DTYPE_F32) launch_join<float>(a, p.cols, mass, st);
         else if (dtype == LLKV_DTYPE_F16) launch_join<_Float16>(a, p.cols, mass, st);
         else launch_join<bf16_t>(a, p.cols, mass, st);
