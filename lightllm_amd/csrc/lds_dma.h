@@ -27,15 +27,23 @@ __device__ inline void dma16(const void* gptr, uint32_t la) {
 
 // The same with a wave-uniform base (scalar registers) and a 32-bit per-lane
 // byte offset (no per-lane 64-bit address arithmetic).
+// NT: a streaming (nontemporal) load.
+template <bool NT = false>
 __device__ inline void dma16_s(const void* sbase, uint32_t voff, uint32_t la) {
     const uint64_t b = (uint64_t)(uintptr_t)sbase;
     // (readfirstlane returns int: widen through uint32_t, not by sign extension)
     const uint64_t bs = ((uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)(b >> 32)) << 32) |
                         (uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)b);
-    asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1"
-                 :
-                 : "v"(voff), "s"(bs), "s"(la)
-                 : "memory", "m0");
+    if constexpr (NT)
+        asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1 nt"
+                     :
+                     : "v"(voff), "s"(bs), "s"(la)
+                     : "memory", "m0");
+    else
+        asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1"
+                     :
+                     : "v"(voff), "s"(bs), "s"(la)
+                     : "memory", "m0");
 }
 
 }  // namespace llkv

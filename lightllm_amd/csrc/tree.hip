@@ -115,47 +115,24 @@ __device__ void slow_columns(const TreeArgs& a, const TreeSeg& sg, int kcols) {
     }
 }
 
-template <typename TT, int D_, int NCT_, bool MASS>
+template <int D_, int NCT_, bool MASS>
 struct FewCols {
-    using T = TT;
+    using T = float;
     static constexpr int D = D_, NCT = NCT_, W = 4;
     static constexpr int kCols = 16 * NCT, kThreads = 64 * W;
     static constexpr bool kMass = MASS, kTeams = false;
-    static constexpr bool k16 = Elem<T>::kDtype != LLKV_DTYPE_F32;
-    static constexpr bool kF16 = Elem<T>::kDtype == LLKV_DTYPE_F16;
     using Ops = ScoreOps<T, D>;
     static constexpr int VH = (D + 63) / 64, DT = 4 * VH, MD = VH;
     // Resident waves per SIMD that the registers are held to (the loads in flight are what
     // bounds a few columns).
-    static constexpr int kWavesPerEU = NCT == 1 ? (D == 64 ? 4 : (D == 96 ? 3 : (D == 128 ? (k16 ? 4 : 3) : 2)))
-                                                : (NCT == 2 && D == 64 ? 3 : (NCT == 2 && D <= 128 ? 2 : 1));
+    static constexpr int kWavesPerEU = NCT == 1 ? (D == 64 ? 4 : (D == 256 ? 1 : (D == 128 && !MASS ? 2 : 3)))
+                                                : (NCT == 2 ? (D == 64 ? 3 : 2) : 1);
 
     struct Smem {
         float acc[W][16][D];
         float ml[W][16][2];   // (max, sum)
         int odd;
     };
-
-    // Q^T operand of one column (as ScoreOps::load_q, with the load outside the choice: inside
-    // it the registers of several column tiles went through scratch memory).
-    __device__ static void load_columns(const T* qrow, bool valid, int g, float scale, typename Ops::QReg (&q)[Ops::NQ]) {
-        if constexpr (k16) {
-#pragma unroll
-            for (int ks = 0; ks < Ops::NQ; ++ks) {
-                const mu32x4 x = *reinterpret_cast<const mu32x4*>(qrow + 32 * ks + 8 * g);
-#pragma unroll
-                for (int e = 0; e < 4; ++e) q[ks][e] = valid ? x[e] : 0u;
-            }
-        } else {
-#pragma unroll
-            for (int cc = 0; cc < D / 16; ++cc) {
-                const float4 x = *reinterpret_cast<const float4*>(qrow + 16 * cc + 4 * g);
-                const float f[4] = {x.x, x.y, x.z, x.w};
-#pragma unroll
-                for (int e = 0; e < 4; ++e) q[4 * cc + e] = valid ? f[e] * scale : 0.0f;
-            }
-        }
-    }
 
     __device__ static void run(const TreeArgs& a, Smem& sm, const TreeSeg& sg) {
         const int lane = threadIdx.x & 63;
@@ -168,7 +145,7 @@ struct FewCols {
         const T* vbase = reinterpret_cast<const T*>(a.v) + (int64_t)sg.kvh * D;
         const int* bt = a.bt + (int64_t)sg.n * a.max_blocks;
 
-        typename Ops::QReg q[NCT][Ops::NQ];
+        float q[NCT][Ops::NQ];
         const int* mrow[NCT];
         mf32x4 o[NCT][DT];
         float m[NCT], l[NCT];
@@ -179,7 +156,13 @@ struct FewCols {
             const int node = valid ? col / G : 0;
             const int64_t row = sg.s.q0 + node;
             const T* qrow = reinterpret_cast<const T*>(a.q) + (row * a.Hq + sg.kvh * G + (valid ? col - node * G : 0)) * D;
-            load_columns(qrow, valid, g, a.scale_log2, q[ct]);
+#pragma unroll
+            for (int cc = 0; cc < D / 16; ++cc) {
+                const float4 x = *reinterpret_cast<const float4*>(qrow + 16 * cc + 4 * g);
+                const float f[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+                for (int e = 0; e < 4; ++e) q[ct][4 * cc + e] = valid ? f[e] * a.scale_log2 : 0.0f;
+            }
             mrow[ct] = MASS ? nullptr : a.mask + row * a.words;
 #pragma unroll
             for (int dt = 0; dt < DT; ++dt) o[ct][dt] = mf32x4{0.f, 0.f, 0.f, 0.f};
@@ -200,25 +183,16 @@ struct FewCols {
             if (pg >= npages) break;
             const int64_t phys = max(__builtin_amdgcn_readlane(tbl, j & 63), 0);
 
-            typename Ops::KReg kr[Ops::NK];
+            float4 kr[Ops::NK];
             Ops::template load_k<false>(kbase + (phys * kPage + c) * row_elems, g, kr);
             float4 vr[VH][4];
-            uint32_t vx[VH][4], vy[VH][4];   // 16-bit V: dims 0, 1 and 2, 3 of a lane's four
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 const T* vp = vbase + (phys * kPage + 4 * g + i) * row_elems + 4 * c;
 #pragma unroll
                 for (int h = 0; h < VH; ++h) {
-                    if (D % 64 != 0 && 64 * h + 4 * c >= D) {   // past the head's last dim
-                        vx[h][i] = vy[h][i] = 0u;
-                        vr[h][i] = make_float4(0.f, 0.f, 0.f, 0.f);
-                    } else if constexpr (k16) {
-                        const mu32x2 x = load_vec<false, mu32x2>(vp + 64 * h);
-                        vx[h][i] = x.x;
-                        vy[h][i] = x.y;
-                    } else {
-                        vr[h][i] = Ops::template load_v4<false>(vp + 64 * h);
-                    }
+                    if (D % 64 != 0 && 64 * h + 4 * c >= D) vr[h][i] = make_float4(0.f, 0.f, 0.f, 0.f);   // past the last dim
+                    else vr[h][i] = Ops::template load_v4<false>(vp + 64 * h);
                 }
             }
 
@@ -235,38 +209,20 @@ struct FewCols {
                     const bool tree = !MASS && p0 + 4 * g + i >= hist && !beyond;
 #pragma unroll
                     for (int h = 0; h < VH; ++h) {
-                        if constexpr (k16) {
-                            odd |= tree && !(finite_bits(vx[h][i], kF16) && finite_bits(vy[h][i], kF16));
-                            vx[h][i] = beyond ? 0u : vx[h][i];
-                            vy[h][i] = beyond ? 0u : vy[h][i];
-                        } else {
-                            odd |= tree && !(isfinite(vr[h][i].x) && isfinite(vr[h][i].y) && isfinite(vr[h][i].z) &&
-                                             isfinite(vr[h][i].w));
-                            if (beyond) vr[h][i] = make_float4(0.f, 0.f, 0.f, 0.f);
-                        }
+                        odd |= tree && !(isfinite(vr[h][i].x) && isfinite(vr[h][i].y) && isfinite(vr[h][i].z) &&
+                                         isfinite(vr[h][i].w));
+                        if (beyond) vr[h][i] = make_float4(0.f, 0.f, 0.f, 0.f);
                     }
                 }
-            }
-
-            mu32x2 av[VH][4];   // V^T operands of the 16-bit product
-            if constexpr (k16) {
-#pragma unroll
-                for (int h = 0; h < VH; ++h)
-#pragma unroll
-                    for (int jj = 0; jj < 4; ++jj) {
-                        const unsigned sel = (jj & 1) ? 0x07060302u : 0x05040100u;
-                        av[h][jj] = jj < 2 ? mu32x2{__builtin_amdgcn_perm(vx[h][1], vx[h][0], sel), __builtin_amdgcn_perm(vx[h][3], vx[h][2], sel)}
-                                           : mu32x2{__builtin_amdgcn_perm(vy[h][1], vy[h][0], sel), __builtin_amdgcn_perm(vy[h][3], vy[h][2], sel)};
-                    }
             }
 
 #pragma unroll
             for (int ct = 0; ct < NCT; ++ct) {
                 const mf32x4 sc = Ops::scores(kr, q[ct], a.scale_log2);
                 float x[4] = {sc[0], sc[1], sc[2], sc[3]};
-                uint32_t seen = ~0u;   // bit i: the lane's key i
                 if (!whole) {
                     const int p4 = p0 + 4 * g;
+                    uint32_t seen = ~0u;   // bit i: the lane's key i
                     if constexpr (!MASS) seen = tree_bits(mrow[ct], a.words, p4 - hist);
                     seen &= L >= p4 + 4 ? ~0u : (1u << max(L - p4, 0)) - 1u;
 #pragma unroll
@@ -279,7 +235,7 @@ struct FewCols {
                                                    p0 + 4 * g) = make_float4(x[0], x[1], x[2], x[3]);
                 }
                 // The running maximum moves only when a column's page exceeds it by more than
-                // 8 (2^8 fits every type), so most pages need no exchange between lanes.
+                // 8, so most pages need no exchange between lanes.
                 const float mt = fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3]));
                 if (__builtin_amdgcn_ballot_w64(mt > m[ct] + 8.0f) != 0) {
                     float mm = fmaxf(mt, __shfl_xor(mt, 16, 64));
@@ -297,33 +253,15 @@ struct FewCols {
                     p[i] = fast_exp2(x[i] - m[ct]);
                     l[ct] += p[i];
                 }
-                if constexpr (k16) {
-                    // P in the pool's type, as the prefill: at most half a step of each weight.
-                    const mu32x2 pb = kF16 ? mu32x2{pack_h2(p[0], p[1]), pack_h2(p[2], p[3])}
-                                           : mu32x2{pack_b2(p[0], p[1]), pack_b2(p[2], p[3])};
 #pragma unroll
-                    for (int h = 0; h < VH; ++h)
+                for (int h = 0; h < VH; ++h)
 #pragma unroll
-                        for (int jj = 0; jj < 4; ++jj) {
-                            mf32x4& acc = o[ct][4 * h + jj];
-                            if constexpr (kF16)
-                                acc = __builtin_amdgcn_mfma_f32_16x16x16f16(__builtin_bit_cast(mf16x4, av[h][jj]),
-                                                                            __builtin_bit_cast(mf16x4, pb), acc, 0, 0, 0);
-                            else
-                                acc = __builtin_amdgcn_mfma_f32_16x16x16bf16_1k(__builtin_bit_cast(ms16x4, av[h][jj]),
-                                                                                __builtin_bit_cast(ms16x4, pb), acc, 0, 0, 0);
-                        }
-                } else {
-#pragma unroll
-                    for (int h = 0; h < VH; ++h)
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) {
-                            o[ct][4 * h + 0] = __builtin_amdgcn_mfma_f32_16x16x4f32(vr[h][i].x, p[i], o[ct][4 * h + 0], 0, 0, 0);
-                            o[ct][4 * h + 1] = __builtin_amdgcn_mfma_f32_16x16x4f32(vr[h][i].y, p[i], o[ct][4 * h + 1], 0, 0, 0);
-                            o[ct][4 * h + 2] = __builtin_amdgcn_mfma_f32_16x16x4f32(vr[h][i].z, p[i], o[ct][4 * h + 2], 0, 0, 0);
-                            o[ct][4 * h + 3] = __builtin_amdgcn_mfma_f32_16x16x4f32(vr[h][i].w, p[i], o[ct][4 * h + 3], 0, 0, 0);
-                        }
-                }
+                    for (int i = 0; i < 4; ++i) {
+                        o[ct][4 * h + 0] = __builtin_amdgcn_mfma_f32_16x16x4f32(vr[h][i].x, p[i], o[ct][4 * h + 0], 0, 0, 0);
+                        o[ct][4 * h + 1] = __builtin_amdgcn_mfma_f32_16x16x4f32(vr[h][i].y, p[i], o[ct][4 * h + 1], 0, 0, 0);
+                        o[ct][4 * h + 2] = __builtin_amdgcn_mfma_f32_16x16x4f32(vr[h][i].z, p[i], o[ct][4 * h + 2], 0, 0, 0);
+                        o[ct][4 * h + 3] = __builtin_amdgcn_mfma_f32_16x16x4f32(vr[h][i].w, p[i], o[ct][4 * h + 3], 0, 0, 0);
+                    }
             }
         }
 
@@ -428,7 +366,7 @@ __device__ inline void score_schedule() {
     }
 }
 
-template <typename TT, int D_, int NCW, int WV, int RING>
+template <typename TT, int D_, int NCW, int WV, int RING, bool MASS = false>
 struct ManyCols {
     using T = TT;
     static constexpr int D = D_, W = WV, R = RING;
@@ -437,11 +375,14 @@ struct ManyCols {
     static constexpr int KT = BN / 16, SS = BN / 32;   // key tiles, key halves of the second product
     static constexpr int KS = D / 32, DT = D / 16;
     static constexpr int CPR = D / 8;                  // 16-byte chunks per row
-    static constexpr int RPB = 64 / CPR;               // rows per 1 KB block
-    static constexpr int RPW = BN / W;                 // rows that a wave loads
-    static constexpr int BPW = RPW / RPB;
+    // Four waves load a quarter of the rows of K and of V each; of eight, four load K's and
+    // four V's, so that a part is whole 1 KB blocks.
+    static constexpr int RPW = BN / 4;
+    static constexpr int BPW = RPW * D * 2 / 1024;
+    static constexpr int kLoads = (W == 4 ? 2 : 1) * BPW;   // of a wave per tile
+    static_assert((W == 4 || W == 8) && RPW * D * 2 % 1024 == 0 && kPage % RPW == 0, "tile parts");
     static constexpr int kWavesPerEU = 2;
-    static constexpr bool kMass = false, kTeams = true;
+    static constexpr bool kMass = MASS, kTeams = !MASS;
     static constexpr uint32_t kOnes = Elem<T>::kDtype == LLKV_DTYPE_F16 ? 0x3C003C00u : 0x3F803F80u;
     static constexpr bool kF16 = Elem<T>::kDtype == LLKV_DTYPE_F16;
 
@@ -451,8 +392,14 @@ struct ManyCols {
         int odd;
     };
 
-    __device__ static int swz(int r) { return ((r & 3) | ((r >> 1) & 0xC)) & (CPR - 1); }
-    __device__ static int at(int row, int d) { return row * D + ((((d >> 3) ^ swz(row)) << 3) | (d & 7)); }
+    // Place of chunk ch of row r, and the chunk at a place: XOR with row bits 0, 1, 3, 4 (the
+    // rows that an operand read takes together differ there), or a rotation by them where a
+    // row's chunks are no power of two.
+    static constexpr bool kXor = (CPR & (CPR - 1)) == 0;
+    __device__ static int bits(int r) { return (r & 3) | ((r >> 1) & 0xC); }
+    __device__ static int place(int r, int ch) { return kXor ? ch ^ (bits(r) & (CPR - 1)) : (ch + bits(r)) % CPR; }
+    __device__ static int chunk(int r, int pl) { return kXor ? pl ^ (bits(r) & (CPR - 1)) : (pl + 16 * CPR - bits(r)) % CPR; }
+    __device__ static int at(int row, int d) { return row * D + (place(row, d >> 3) << 3 | (d & 7)); }
 
     __device__ static void run(const TreeArgs& a, Smem& sm, const TreeSeg& sg) {
         const int tid = threadIdx.x, lane = tid & 63;
@@ -461,34 +408,37 @@ struct ManyCols {
         const int G = a.Hq / a.Hkv;
         const int L = sg.s.L, hist = sg.s.hist;
         const uint32_t row_bytes = (uint32_t)(a.Hkv * D * sizeof(T));
-        const char* kb = reinterpret_cast<const char*>(reinterpret_cast<const T*>(a.k) + (int64_t)sg.kvh * D);
-        const char* vb = reinterpret_cast<const char*>(reinterpret_cast<const T*>(a.v) + (int64_t)sg.kvh * D);
+        const char* kp = reinterpret_cast<const char*>(reinterpret_cast<const T*>(a.k) + (int64_t)sg.kvh * D);
+        const char* vp = reinterpret_cast<const char*>(reinterpret_cast<const T*>(a.v) + (int64_t)sg.kvh * D);
         const int* bt = a.bt + (int64_t)sg.n * a.max_blocks;
         const int last_page = L > 0 ? (L - 1) / kPage : 0;
         // keys [begin, stop) in tiles of BN
         const int begin = sg.t0 * kTreeTile;
         const int tiles = (min(sg.t1 * kTreeTile, L) - begin + BN - 1) / BN;   // 0 or less: no key
 
-        // The wave's rows of a tile: one page or a part of one.
+        // The wave's rows of a tile, a page or a part of one: 16-byte units u of them, 64 per block.
         constexpr uint32_t kTileBytes = BN * D * 2;
-        uint32_t off[BPW], lds_k[BPW], lds_v[BPW];
+        const int part = RPW * (w & 3);   // first row
+        const bool loads_v = W == 8 && w >= 4;
+        uint32_t off[BPW], to_k[BPW], to_v[BPW];
 #pragma unroll
-        for (int j = 0; j < BPW; ++j) {
-            const int r = RPW * w + j * RPB + lane / CPR;   // row of the tile
-            off[j] = (uint32_t)(r % kPage) * row_bytes + (uint32_t)(((lane % CPR) ^ swz(r)) * 16);
-            lds_k[j] = lds_addr(&sm.k[0][(RPW * w + j * RPB) * D]);
-            lds_v[j] = lds_addr(&sm.v[0][(RPW * w + j * RPB) * D]);
+        for (int i = 0; i < BPW; ++i) {
+            const int u = 64 * i + lane, r = part + u / CPR;
+            off[i] = (uint32_t)(r % kPage) * row_bytes + (uint32_t)chunk(r, u % CPR) * 16u;
+            to_k[i] = lds_addr((loads_v ? sm.v[0] : sm.k[0]) + part * D + 512 * i);
+            to_v[i] = lds_addr(sm.v[0] + part * D + 512 * i);
         }
+        const char* const kb = loads_v ? vp : kp;
         int tbl = 0;   // page ids of the wave's next 64 tiles, one per lane
         auto load_tile = [&](int j) {
-            if ((j & 63) == 0) tbl = bt[min((begin + (j + lane) * BN + RPW * w) / kPage, last_page)];
+            if ((j & 63) == 0) tbl = bt[min((begin + (j + lane) * BN + part) / kPage, last_page)];
             const int phys = max(__builtin_amdgcn_readlane(tbl, j & 63), 0);
             const uint64_t base = (uint64_t)(uint32_t)phys * row_bytes * kPage;
             const uint32_t to = (uint32_t)(j % R) * kTileBytes;
 #pragma unroll
             for (int i = 0; i < BPW; ++i) {
-                dma16_s(kb + base, off[i], lds_k[i] + to);
-                dma16_s(vb + base, off[i], lds_v[i] + to);
+                dma16_s<MASS>(kb + base, off[i], to_k[i] + to);
+                if constexpr (W == 4) dma16_s(vp + base, off[i], to_v[i] + to);
             }
         };
 #pragma unroll
@@ -509,8 +459,10 @@ struct ManyCols {
         const uint32_t flip = a.scale_log2 < 0.0f ? 0x80008000u : 0u;
         mu32x4 q[NCW][KS];
         const int* mrow[NCW];
+        // Row sums: of the rounded weights, as O's products take them, by a tile of ones; of
+        // kept weights, which the log-sum-exp normalises in 32 bits, of the weights themselves.
         mf32x4 o[NCW][DT], osum[NCW];
-        float m[NCW];
+        float m[NCW], l[NCW];
 #pragma unroll
         for (int nt = 0; nt < NCW; ++nt) {
             const int col = sg.c0 + (w * NCW + nt) * 16 + c;
@@ -523,19 +475,21 @@ struct ManyCols {
                 const mu32x4 x = *reinterpret_cast<const mu32x4*>(qrow + 32 * ks + 8 * g);
                 q[nt][ks] = valid ? x ^ flip : mu32x4{0u, 0u, 0u, 0u};
             }
-            mrow[nt] = a.mask + row * a.words;
+            mrow[nt] = MASS ? nullptr : a.mask + row * a.words;
 #pragma unroll
             for (int dt = 0; dt < DT; ++dt) o[nt][dt] = mf32x4{0.f, 0.f, 0.f, 0.f};
             osum[nt] = mf32x4{0.f, 0.f, 0.f, 0.f};
             m[nt] = kNegBig;
+            l[nt] = 0.0f;
         }
         const mu32x4 ones = {kOnes, kOnes, kOnes, kOnes};
         bool odd = false;
+        const bool idle = sg.c0 + w * NCW * 16 >= sg.cols;   // the wave has no column: it loads and waits only
 
         for (int j = 0; j < tiles; ++j) {
             // This wave's part of tile j is in LDS: all loads but those of the tiles after it.
             const int after = tiles - 1 - j;
-            constexpr int kAll = vmcnt_imm(2 * BPW * (R - 2)), kLess = vmcnt_imm(R > 2 ? 2 * BPW * (R - 3) : 0);
+            constexpr int kAll = vmcnt_imm(kLoads * (R - 2)), kLess = vmcnt_imm(R > 2 ? kLoads * (R - 3) : 0);
             if (after >= R - 2) __builtin_amdgcn_s_waitcnt(kAll);
             else if (after == R - 3) __builtin_amdgcn_s_waitcnt(kLess);
             else __builtin_amdgcn_s_waitcnt(vmcnt_imm(0));
@@ -561,11 +515,12 @@ struct ManyCols {
                     const int r = i / CPR;
                     mu32x4& x = *reinterpret_cast<mu32x4*>(vt_lds + i * 8);
                     if (key0 + r >= L) x = mu32x4{0u, 0u, 0u, 0u};
-                    else if (key0 + r >= hist)
+                    else if (!MASS && key0 + r >= hist)
                         odd |= !(finite_bits(x.x, kF16) && finite_bits(x.y, kF16) && finite_bits(x.z, kF16) && finite_bits(x.w, kF16));
                 }
                 lds_barrier();
             }
+            if (idle) continue;   // (uniform over the wave)
             __builtin_amdgcn_sched_barrier(0);   // the next tile's loads are issued first
             if constexpr (D >= 128) __builtin_amdgcn_s_setprio(1);
             // S^T = K Q^T, the K operands of k-step ks + 1 read behind the products of ks
@@ -602,10 +557,20 @@ struct ManyCols {
 #pragma unroll
                     for (int kt = 0; kt < KT; ++kt) {
                         const int k4 = key0 + 32 * (kt >> 1) + 8 * g + 4 * (kt & 1);
-                        uint32_t seen = tree_bits(mrow[nt], a.words, k4 - hist);
+                        uint32_t seen = ~0u;
+                        if constexpr (!MASS) seen = tree_bits(mrow[nt], a.words, k4 - hist);
                         seen &= L >= k4 + 4 ? ~0u : (1u << max(L - k4, 0)) - 1u;
 #pragma unroll
                         for (int i = 0; i < 4; ++i) s[kt][nt][i] = seen >> i & 1u ? s[kt][nt][i] : -INFINITY;
+                    }
+                }
+                if constexpr (MASS) {
+                    const int col = sg.c0 + (w * NCW + nt) * 16 + c;
+                    float* sc = a.scores + ((int64_t)(sg.n * a.Hkv + sg.kvh) * G + col) * a.score_stride + key0 + 8 * g;
+                    if (col < sg.cols) {
+#pragma unroll
+                        for (int kt = 0; kt < KT; ++kt)
+                            *reinterpret_cast<mf32x4*>(sc + 32 * (kt >> 1) + 4 * (kt & 1)) = s[kt][nt] * scale;
                     }
                 }
                 float v = -INFINITY;
@@ -625,7 +590,8 @@ struct ManyCols {
                     const float mnew = fmaxf(m[nt], v);
                     const float corr = fast_exp2(m[nt] - mnew);
                     m[nt] = mnew;
-                    osum[nt] *= corr;
+                    if constexpr (MASS) l[nt] *= corr;
+                    else osum[nt] *= corr;
 #pragma unroll
                     for (int dt = 0; dt < DT; ++dt) o[nt][dt] *= corr;
                 }
@@ -633,7 +599,11 @@ struct ManyCols {
             // P in the pool's type (half a step of each weight, as the prefill), its row sums by
             // the same rounded weights; O^T += V^T P^T.  The exponentials of the second 32 keys
             // are spread between the products of the first.
-            auto weight = [&](int ss, int nt, int i) { return fast_exp2(fmaf(s[2 * ss + (i >> 2)][nt][i & 3], scale, -m[nt])); };
+            auto weight = [&](int ss, int nt, int i) {
+                const float p = fast_exp2(fmaf(s[2 * ss + (i >> 2)][nt][i & 3], scale, -m[nt]));
+                if constexpr (MASS) l[nt] += p;
+                return p;
+            };
             auto pack = [&](const float* e) {
                 return mu32x4{pack_pair<T>(e[0], e[1]), pack_pair<T>(e[2], e[3]), pack_pair<T>(e[4], e[5]), pack_pair<T>(e[6], e[7])};
             };
@@ -656,7 +626,7 @@ struct ManyCols {
                 if (dt < DT) {
                     o[nt][dt] = mma32<T>(va[dt], p[nt], o[nt][dt]);
                     if (SS == 2 && nt == NCW - 1) va[dt] = v_operand(dt, 1);
-                } else {
+                } else if constexpr (!MASS) {
                     osum[nt] = mma32<T>(ones, p[nt], osum[nt]);
                 }
                 if constexpr (SS == 2) {
@@ -672,19 +642,28 @@ struct ManyCols {
                 for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
                     for (int nt = 0; nt < NCW; ++nt) o[nt][dt] = mma32<T>(va[dt], p[nt], o[nt][dt]);
+                if constexpr (!MASS) {
 #pragma unroll
-                for (int nt = 0; nt < NCW; ++nt) osum[nt] = mma32<T>(ones, p[nt], osum[nt]);
+                    for (int nt = 0; nt < NCW; ++nt) osum[nt] = mma32<T>(ones, p[nt], osum[nt]);
+                }
             }
         }
-        if (odd_segment(sm.odd, odd)) {
+        if constexpr (MASS) {
+            lds_barrier();   // the last tile has been read: the next segment loads into the ring
+        } else if (odd_segment(sm.odd, odd)) {
             slow_columns<T, D>(a, sg, kCols);
             return;
         }
 #pragma unroll
         for (int nt = 0; nt < NCW; ++nt) {
             const int cc = (w * NCW + nt) * 16 + c, col = sg.c0 + cc;
+            float sum = osum[nt][0];
+            if constexpr (MASS) {
+                sum = l[nt] + __shfl_xor(l[nt], 16, 64);
+                sum += __shfl_xor(sum, 32, 64);
+            }
             if (col >= sg.cols) continue;
-            const float sum = osum[nt][0], inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+            const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
             const int node = col / G;
             T* out = reinterpret_cast<T*>(a.out) + ((int64_t)(sg.s.q0 + node) * a.Hq + sg.kvh * G + (col - node * G)) * D;
             const int64_t part = (int64_t)sg.slot * kCols + cc;
@@ -697,7 +676,11 @@ struct ManyCols {
                 else
                     *reinterpret_cast<mf32x4*>(a.part_o + part * D + d) = x;
             }
-            if (g == 0 && !sg.direct) a.part_lse[part] = sum == 0.0f ? -INFINITY : m[nt] + fast_log2(sum);
+            if (g == 0) {
+                const float lse = sum == 0.0f ? -INFINITY : m[nt] + fast_log2(sum);
+                if (!sg.direct) a.part_lse[part] = lse;
+                else if constexpr (MASS) a.lse[(int64_t)sg.n * a.Hq + sg.kvh * G + (col - node * G)] = lse;
+            }
         }
     }
 };
@@ -765,86 +748,126 @@ __global__ __launch_bounds__(B::kThreads) __attribute__((amdgpu_waves_per_eu(B::
 // Slot of part j of a cut unit that begins in work-group w.
 __device__ inline int part_slot(int w, int first_slot, int step, int j) { return j == 0 ? first_slot : 2 * (w + j * step); }
 
-// Log-sum-exp join of one column's parts: a wave, lane owning dims lane + 64 i.
-// Returns the column's log2-sum-exp2.
-template <typename T, int MD>
-__device__ inline float join_parts(const TreeArgs& a, int cols, int w, int first_slot, int step, int parts, int col, T* out) {
-    constexpr int kBatch = 4;
-    const int lane = threadIdx.x & 63;
-    float M = -INFINITY, sum = 0.0f, o[MD];
+// Log-sum-exp join of a cut unit's parts, columns first, first + stride .. by one
+// work-group: LR lanes hold a row, 16 bytes each, and as many rows as the work-group
+// has lanes for are read at once, of one column's parts first.  (A wave per
+// column with its parts one after the other: 54 us for 8 units of 64 columns of 64
+// parts, more than the 17 us of the kernel that wrote them.)  out_row(c): the
+// output row of column c.
+struct JoinSmem {
+    mf32x4 o[256];
+    float ml[64][2];   // (max, sum) per row
+};
+
+template <typename T, int LR, class OutRow>
+__device__ inline void join_columns(const TreeArgs& a, JoinSmem& sm, int cols, int w, const TreeCut& u, int first, int stride,
+                                    OutRow out_row) {
+    constexpr int RW = 256 / LR;   // rows at once
+    constexpr int kBatch = 4;      // rows in flight per lane
+    const int r = threadIdx.x / LR, l = threadIdx.x % LR;
+    int sp = 1;                    // rows of one column: a lane takes kBatch of its parts at once
+    while (sp * kBatch < u.parts && sp < RW) sp *= 2;
+    const int cpw = RW / sp, sub = r % sp;
+    const int here = min(cols, u.cols - u.c0);
+    const bool lane_on = 4 * l < a.D;
+    for (int c0 = first * cpw; c0 < here; c0 += stride * cpw) {   // uniform
+        const int c = c0 + r / sp;
+        float M = -INFINITY, sum = 0.0f;
+        mf32x4 o = {0.f, 0.f, 0.f, 0.f};
+        if (c < here) {
+            for (int j0 = sub; j0 < u.parts; j0 += kBatch * sp) {
+                float lv[kBatch];
+                mf32x4 pv[kBatch];
 #pragma unroll
-    for (int i = 0; i < MD; ++i) o[i] = 0.0f;
-    for (int j0 = 0; j0 < parts; j0 += kBatch) {
-        float lv[kBatch], pv[kBatch][MD];
+                for (int b = 0; b < kBatch; ++b) {
+                    const int j = j0 + b * sp;
+                    const bool ok = j < u.parts;
+                    const int64_t row = (int64_t)part_slot(w, u.slot, u.step, ok ? j : j0) * cols + c;
+                    lv[b] = ok ? a.part_lse[row] : -INFINITY;
+                    pv[b] = *reinterpret_cast<const mf32x4*>(a.part_o + row * a.D + (lane_on ? 4 * l : 0));
+                }
+                float mb = M;
 #pragma unroll
-        for (int j = 0; j < kBatch; ++j) {
-            const bool ok = j0 + j < parts;
-            const int64_t row = (int64_t)part_slot(w, first_slot, step, j0 + (ok ? j : 0)) * cols + col;
-            lv[j] = ok ? a.part_lse[row] : -INFINITY;
+                for (int b = 0; b < kBatch; ++b) mb = fmaxf(mb, lv[b]);
+                if (mb == -INFINITY) continue;   // no key seen so far
+                const float sc = fast_exp2(M - mb);
+                sum *= sc;
+                o *= sc;
 #pragma unroll
-            for (int i = 0; i < MD; ++i) pv[j][i] = a.part_o[row * a.D + min(lane + 64 * i, a.D - 1)];
+                for (int b = 0; b < kBatch; ++b) {
+                    const float f = fast_exp2(lv[b] - mb);
+                    sum += f;
+                    o += f * pv[b];
+                }
+                M = mb;
+            }
         }
-        float mb = M;
-#pragma unroll
-        for (int j = 0; j < kBatch; ++j) mb = fmaxf(mb, lv[j]);
-        if (mb == -INFINITY) continue;   // no key seen so far
-        const float sc = fast_exp2(M - mb);
-        sum *= sc;
-#pragma unroll
-        for (int i = 0; i < MD; ++i) o[i] *= sc;
-#pragma unroll
-        for (int j = 0; j < kBatch; ++j) {
-            const float f = fast_exp2(lv[j] - mb);
-            sum += f;
-#pragma unroll
-            for (int i = 0; i < MD; ++i) o[i] = fmaf(f, pv[j][i], o[i]);
+        if (sp > 1) {   // uniform
+            sm.o[threadIdx.x] = o;
+            if (l == 0) {
+                sm.ml[r][0] = M;
+                sm.ml[r][1] = sum;
+            }
+            __syncthreads();
+            if (sub == 0) {
+                float top = M;
+                for (int i = 1; i < sp; ++i) top = fmaxf(top, sm.ml[r + i][0]);
+                if (top > -INFINITY) {
+                    float f = fast_exp2(M - top);
+                    sum *= f;
+                    o *= f;
+                    for (int i = 1; i < sp; ++i) {
+                        f = fast_exp2(sm.ml[r + i][0] - top);
+                        sum = fmaf(f, sm.ml[r + i][1], sum);
+                        o += f * sm.o[threadIdx.x + i * LR];
+                    }
+                }
+            }
+            __syncthreads();
         }
-        M = mb;
+        if (sub == 0 && c < here && lane_on) {
+            o *= sum == 0.0f ? 0.0f : 1.0f / sum;
+            T* out = out_row(c) + 4 * l;
+            if constexpr (sizeof(T) == 4) *reinterpret_cast<mf32x4*>(out) = o;
+            else *reinterpret_cast<mu32x2*>(out) = mu32x2{pack_pair<T>(o[0], o[1]), pack_pair<T>(o[2], o[3])};
+        }
     }
-    const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
-#pragma unroll
-    for (int i = 0; i < MD; ++i)
-        if (lane + 64 * i < a.D) out[lane + 64 * i] = Elem<T>::from_f32(o[i] * inv);
-    return sum == 0.0f ? -INFINITY : M + fast_log2(sum);
 }
 
-// Grid (shares, kJoinSlices), a wave per column at a time.
-constexpr int kJoinSlices = 16;
+// Grid (work-groups of the first kernel, slices of the columns).
 
-template <typename T, int MD>
+template <typename T, int LR>
 __global__ __launch_bounds__(256) void tree_join_kernel(TreeArgs a, int cols) {
-    const int w = blockIdx.x;
-    const TreeCut u = a.cuts[w];
+    __shared__ JoinSmem sm;
+    const TreeCut u = a.cuts[blockIdx.x];
     if (u.parts == 0) return;
     const int G = a.Hq / a.Hkv;
-    for (int c = blockIdx.y * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6); c < cols; c += 4 * kJoinSlices) {
-        const int col = u.c0 + c;
-        if (col >= u.cols) return;
-        const int node = col / G;
-        T* out = reinterpret_cast<T*>(a.out) + ((int64_t)(u.q0 + node) * a.Hq + u.kvh * G + (col - node * G)) * a.D;
-        join_parts<T, MD>(a, cols, w, u.slot, u.step, u.parts, c, out);
-    }
+    join_columns<T, LR>(a, sm, cols, blockIdx.x, u, blockIdx.y, gridDim.y, [&](int c) {
+        const int col = u.c0 + c, node = col / G;
+        return reinterpret_cast<T*>(a.out) + ((int64_t)(u.q0 + node) * a.Hq + u.kvh * G + (col - node * G)) * a.D;
+    });
 }
 
-// Kept weights: grid (key blocks of kMassKeys, Hkv, N), four keys per thread.  Each
-// work-group takes the unit's log2-sum-exp2 per query head (joining the parts of
-// a cut unit; the first key block joins its output rows as well), then adds
-// sum over the group's heads of 2^(score - lse) to its keys' totals.  The first
-// heads' scores are loaded before the log-sum-exps are known.
+// Kept weights: grid (1 + key blocks of kMassKeys, Hkv, N).  Block 0 joins the
+// output rows of a cut unit.  The others take the unit's log2-sum-exp2 per query
+// head (of a cut unit, from its parts) and add
+// sum over the group's heads of 2^(score - lse) to their keys' totals, four keys
+// per thread; the first heads' scores are loaded before the log-sum-exps are known.
 constexpr int kMassKeys = 1024;
 constexpr int kMassGroup = 64;   // query heads of a kv head, at most
 constexpr int kMassAhead = 8;    // heads whose scores are in flight
 
-template <typename T, int MD>
+template <typename T, int LR>
 __global__ __launch_bounds__(256) void mass_join_kernel(TreeArgs a, int cols) {
+    __shared__ JoinSmem sm;
     __shared__ float lse[kMassGroup];
     const int n = blockIdx.z, kvh = blockIdx.y, G = a.Hq / a.Hkv;
     const TreeSeq s = tree_seq(a, n);
-    const int first = blockIdx.x * kMassKeys;
-    if (first > 0 && first >= s.L) return;
+    const int first = ((int)blockIdx.x - 1) * kMassKeys;
+    if (first >= s.L) return;
     const int lane = threadIdx.x & 63, wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int j0 = first + 4 * (int)threadIdx.x;
-    const bool mine = j0 < s.L;
+    const bool keys = first >= 0;
     const float* sc = a.scores + ((int64_t)n * a.Hkv + kvh) * G * a.score_stride + j0;
     float* mass = a.mass + n * a.mass_bs + kvh * a.mass_hs + j0;
     mf32x4 x[kMassAhead];
@@ -852,30 +875,35 @@ __global__ __launch_bounds__(256) void mass_join_kernel(TreeArgs a, int cols) {
     auto load = [&](int h0) {
 #pragma unroll
         for (int h = 0; h < kMassAhead; ++h)
-            if (mine && h0 + h < G) x[h] = *reinterpret_cast<const mf32x4*>(sc + (h0 + h) * a.score_stride);
+            if (j0 < s.L && h0 + h < G) x[h] = *reinterpret_cast<const mf32x4*>(sc + (h0 + h) * a.score_stride);
     };
-    load(0);
+    if (keys) {
+        load(0);
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
-        if (j0 + i < s.L) old[i] = mass[i];
-
+        for (int i = 0; i < 4; ++i)
+            if (j0 + i < s.L) old[i] = mass[i];
+    }
     const int64_t T_ = a.Hkv * a.plan[a.N];
-    const int nwg = tree_shares(a, T_);
+    const int nwg = (int)min(T_, (int64_t)a.nwg);
     const int tiles = tree_tiles(s);
     const int64_t begin = a.Hkv * a.plan[n] + (int64_t)kvh * tiles, end = begin + tiles;   // one column block
-    const int w = (int)wg_of(begin, T_, nwg), last = (int)wg_of(end - 1, T_, nwg);
-    const int slot = 2 * w + (begin == share_begin(w, T_, nwg) ? 0 : 1);
+    const int w = (int)wg_of(begin, T_, nwg), parts = (int)wg_of(end - 1, T_, nwg) - w + 1;
+    const TreeCut u{n, G, 0, kvh, 2 * w + (begin == share_begin(w, T_, nwg) ? 0 : 1), parts, 1};
+    if (!keys) {
+        if (parts > 1)
+            join_columns<T, LR>(a, sm, cols, w, u, 0, 1, [&](int c) {
+                return reinterpret_cast<T*>(a.out) + ((int64_t)n * a.Hq + kvh * G + c) * a.D;
+            });
+        return;
+    }
     for (int c = wv; c < G; c += 4) {
-        const int64_t hq = (int64_t)n * a.Hq + kvh * G + c;
         float v;
-        if (w == last) {
-            v = a.lse[hq];
-        } else if (blockIdx.x == 0) {
-            v = join_parts<T, MD>(a, cols, w, slot, 1, last - w + 1, c, reinterpret_cast<T*>(a.out) + hq * a.D);
+        if (parts == 1) {
+            v = a.lse[(int64_t)n * a.Hq + kvh * G + c];
         } else {
             float M = -INFINITY, sum = 0.0f;
-            for (int j = lane; j < last - w + 1; j += 64) {
-                const float y = a.part_lse[(int64_t)part_slot(w, slot, 1, j) * cols + c];
+            for (int j = lane; j < parts; j += 64) {
+                const float y = a.part_lse[(int64_t)part_slot(w, u.slot, 1, j) * cols + c];
                 const float mb = fmaxf(M, y);
                 if (mb == -INFINITY) continue;
                 sum = sum * fast_exp2(M - mb) + fast_exp2(y - mb);
@@ -1055,34 +1083,38 @@ TreeChoice choice() {
     return TreeChoice{tree_kernel<B>, B::kCols, B::kThreads};
 }
 
-// Columns by the most that a sequence of the call has (cols): one unit where the
-// registers allow it, since a second one reads K and V again; units of 16 columns
-// where the call does not fill the GPU otherwise (tiles: of all (sequence, kv
-// head) pairs).
-template <typename T, int D>
-TreeChoice choose(int64_t cols, int64_t tiles, bool mass) {
-    constexpr bool k16 = Elem<T>::kDtype != LLKV_DTYPE_F32;
-    if (mass) {   // one unit per (sequence, kv head); wider groups take the generic kernel
-        if (cols <= 16) return choice<FewCols<T, D, 1, true>>();
-        if constexpr (D <= 128 || k16)
-            if (cols <= 32) return choice<FewCols<T, D, 2, true>>();
+// By the most columns that a sequence of the call has and the tiles of all
+// (sequence, kv head) pairs.  mass: one unit per (sequence, kv head); wider groups
+// than the kernels' columns take the generic one.
+template <int D>
+TreeChoice choose_f32(int64_t cols, int64_t tiles, bool mass) {
+    if (mass) {
+        if (cols <= 16) return choice<FewCols<D, 1, true>>();
+        if constexpr (D < 256)
+            if (cols <= 32) return choice<FewCols<D, 2, true>>();
         return TreeChoice();
     }
-    if (cols <= 16 || tiles * ((cols + 63) / 64) < device_cus() / 2) return choice<FewCols<T, D, 1, false>>();
-    if constexpr (k16 && D != 96) {
-        if constexpr (D <= 128) {
-            if (cols <= 32) return choice<FewCols<T, D, 2, false>>();
-            if (cols > 128) return choice<ManyCols<T, D, 2, 8, 4>>();
-            if (cols > 64) return choice<ManyCols<T, D, 2, 4, 2>>();
-        }
-        return choice<ManyCols<T, D, 1, 4, 2>>();
-    } else if constexpr (D == 256) {
-        return choice<FewCols<T, D, 1, false>>();
-    } else {
-        if constexpr (k16 || D == 64)
-            if (cols > 32) return choice<FewCols<T, D, 4, false>>();
-        return choice<FewCols<T, D, 2, false>>();
-    }
+    // 16 columns also where wider units would not fill the GPU
+    if (D == 256 || cols <= 16 || tiles * ((cols + 63) / 64) < device_cus() / 2) return choice<FewCols<D, 1, false>>();
+    if constexpr (D == 64)
+        if (cols > 32) return choice<FewCols<D, 4, false>>();
+    if constexpr (D < 256) return choice<FewCols<D, 2, false>>();
+    return TreeChoice();
+}
+
+template <typename T, int D>
+TreeChoice choose_16(int64_t cols, int64_t, bool mass) {
+    if (mass) return choice<ManyCols<T, D, 1, 8, 4, true>>();
+    if constexpr (D <= 128)
+        if (cols > 128) return choice<ManyCols<T, D, 2, 8, 4>>();
+    if (cols > 64) return choice<ManyCols<T, D, 1, 8, 4>>();
+    return choice<ManyCols<T, D, 1, 4, 2>>();
+}
+
+template <typename T, int D>
+TreeChoice choose(int64_t cols, int64_t tiles, bool mass) {
+    if constexpr (Elem<T>::kDtype == LLKV_DTYPE_F32) return choose_f32<D>(cols, tiles, mass);
+    else return choose_16<T, D>(cols, tiles, mass);
 }
 
 template <typename T>
@@ -1099,20 +1131,21 @@ TreeChoice choose(int dtype, int D, int64_t cols, int64_t tiles, bool mass) {
     return choose<bf16_t>(D, cols, tiles, mass);
 }
 
+template <typename T, int LR>
+void launch_join(const TreeArgs& a, int cols, bool mass, hipStream_t st) {
+    if (mass) {
+        const dim3 grid((unsigned)(1 + (a.max_len + kMassKeys - 1) / kMassKeys), a.Hkv, a.N);
+        mass_join_kernel<T, LR><<<grid, 256, 0, st>>>(a, cols);
+    } else {
+        tree_join_kernel<T, LR><<<dim3(a.nwg, cols / 8), 256, 0, st>>>(a, cols);
+    }
+}
+
 template <typename T>
 void launch_join(const TreeArgs& a, int cols, bool mass, hipStream_t st) {
-    const int md = (a.D + 63) / 64;
-    if (mass) {
-        const dim3 grid((unsigned)std::max(1, (a.max_len + kMassKeys - 1) / kMassKeys), a.Hkv, a.N);
-        if (md == 1) mass_join_kernel<T, 1><<<grid, 256, 0, st>>>(a, cols);
-        else if (md == 2) mass_join_kernel<T, 2><<<grid, 256, 0, st>>>(a, cols);
-        else mass_join_kernel<T, 4><<<grid, 256, 0, st>>>(a, cols);
-        return;
-    }
-    const dim3 grid(a.nwg, kJoinSlices);
-    if (md == 1) tree_join_kernel<T, 1><<<grid, 256, 0, st>>>(a, cols);
-    else if (md == 2) tree_join_kernel<T, 2><<<grid, 256, 0, st>>>(a, cols);
-    else tree_join_kernel<T, 4><<<grid, 256, 0, st>>>(a, cols);
+    if (a.D == 64) launch_join<T, 16>(a, cols, mass, st);
+    else if (a.D <= 128) launch_join<T, 32>(a, cols, mass, st);
+    else launch_join<T, 64>(a, cols, mass, st);
 }
 
 size_t up256(size_t n) { return (n + 255) & ~(size_t)255; }

@@ -180,7 +180,4 @@ __device__ inline TreeUnit tree_unit(const TreeArgs& a, const int64_t* P, int n,
     return u;
 }
 
-// Work-groups that have a share: every one holds at least one tile.
-__device__ inline int tree_shares(const TreeArgs& a, int64_t T) { return (int)(T < a.nwg ? T : a.nwg); }
-
 }  // namespace llkv
