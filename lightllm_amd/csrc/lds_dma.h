@@ -6,6 +6,9 @@
 
 namespace llkv {
 
+// S_WAITCNT's operand for at most n vector memory operations left, the other counters free.
+constexpr int vmcnt_imm(int n) { return 0x3F70 | (n & 15) | (n >> 4) << 14; }
+
 // Direct-to-LDS load of 16 bytes per lane: lane L's bytes land at LDS address
 // lds + 16 L (lds uniform over the wave).  Issued as inline assembly, so that
 // the compiler, which cannot tell the two tile buffers apart, does not wait for

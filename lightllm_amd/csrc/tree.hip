@@ -120,13 +120,12 @@ struct FewCols {
     using T = float;
     static constexpr int D = D_, NCT = NCT_, W = 4;
     static constexpr int kCols = 16 * NCT, kThreads = 64 * W;
-    static constexpr bool kMass = MASS, kTeams = false;
+    static constexpr bool kMass = MASS, kTeams = false, kStreams = false;
     using Ops = ScoreOps<T, D>;
     static constexpr int VH = (D + 63) / 64, DT = 4 * VH, MD = VH;
     // Resident waves per SIMD that the registers are held to (the loads in flight are what
     // bounds a few columns).
-    static constexpr int kWavesPerEU = NCT == 1 ? (D == 64 ? 4 : (D == 256 ? 1 : (D == 128 && !MASS ? 2 : 3)))
-                                                : (NCT == 2 ? (D == 64 ? 3 : 2) : 1);
+    static constexpr int kWavesPerEU = NCT == 1 ? (D == 64 ? 4 : (D == 256 ? 1 : (D == 128 && !MASS ? 2 : 3))) : (D == 64 ? 3 : 2);
 
     struct Smem {
         float acc[W][16][D];
@@ -329,9 +328,6 @@ struct FewCols {
     }
 };
 
-// S_WAITCNT's operand for at most n vector memory operations left, the other counters free.
-constexpr int vmcnt_imm(int n) { return 0x3F70 | (n & 15) | (n >> 4) << 14; }
-
 // V_MFMA_F32_16X16X32 of a 16-bit type.
 template <typename T>
 __device__ inline mf32x4 mma32(const mu32x4& x, const mu32x4& y, mf32x4 c) {
@@ -382,7 +378,7 @@ struct ManyCols {
     static constexpr int kLoads = (W == 4 ? 2 : 1) * BPW;   // of a wave per tile
     static_assert((W == 4 || W == 8) && RPW * D * 2 % 1024 == 0 && kPage % RPW == 0, "tile parts");
     static constexpr int kWavesPerEU = 2;
-    static constexpr bool kMass = MASS, kTeams = !MASS;
+    static constexpr bool kMass = MASS, kTeams = !MASS, kStreams = true;
     static constexpr uint32_t kOnes = Elem<T>::kDtype == LLKV_DTYPE_F16 ? 0x3C003C00u : 0x3F803F80u;
     static constexpr bool kF16 = Elem<T>::kDtype == LLKV_DTYPE_F16;
 
@@ -437,8 +433,13 @@ struct ManyCols {
             const uint32_t to = (uint32_t)(j % R) * kTileBytes;
 #pragma unroll
             for (int i = 0; i < BPW; ++i) {
-                dma16_s<MASS>(kb + base, off[i], to_k[i] + to);
-                if constexpr (W == 4) dma16_s(vp + base, off[i], to_v[i] + to);
+                if (sg.stream) {   // (uniform)
+                    dma16_s<true>(kb + base, off[i], to_k[i] + to);
+                    if constexpr (W == 4) dma16_s<true>(vp + base, off[i], to_v[i] + to);
+                } else {
+                    dma16_s(kb + base, off[i], to_k[i] + to);
+                    if constexpr (W == 4) dma16_s(vp + base, off[i], to_v[i] + to);
+                }
             }
         };
 #pragma unroll
@@ -685,7 +686,43 @@ struct ManyCols {
     }
 };
 
+// Log-sum-exp join of a cut unit's parts.  LR lanes hold a row, 16 bytes each, and a
+// work-group as many rows as it has lanes for: of a column's parts kBatch per lane
+// and as many lane groups as that takes (parts_groups), so that most joins are one
+// round trip; the rest are other columns (join_width).  (A wave per column with its
+// parts one after the other: 54 us for 8 units of 64 columns of 64 parts, 17 us the
+// kernel that wrote them.)
+constexpr int kBatch = 4;
+
+// Lanes of a row.
+constexpr int join_lanes(int D) { return D <= 64 ? 16 : (D <= 128 ? 32 : 64); }
+
+template <int LR>
+__device__ inline int part_groups(int parts) {
+    int sp = 1;
+    while (sp * kBatch < parts && sp < 256 / LR) sp *= 2;
+    return sp;
+}
+
+// Columns at once.
+template <int LR>
+__device__ inline int join_width(int parts) { return 256 / LR / part_groups<LR>(parts); }
+
 constexpr int kXcds = 8;
+constexpr int64_t kTreeStreamBytes = 192ll << 20;
+
+// Whether page pg of sequence n is another sequence's too: a prefix lies at the same
+// place of each table, so one entry per sequence tells.  The same in every wave.
+__device__ inline bool shared_page(const TreeArgs& a, int n, int pg) {
+    pg = min(pg, a.max_blocks - 1);
+    const int id = a.bt[(int64_t)n * a.max_blocks + pg];
+    bool same = false;
+    for (int j = threadIdx.x & 63; j < a.N; j += 64) {
+        const int l = a.lens[j];
+        same |= (a.bt[(int64_t)j * a.max_blocks + pg] == id) & (l > pg * kPage) & (j != n);
+    }
+    return __builtin_amdgcn_ballot_w64(same) != 0;
+}
 
 template <class B>
 __global__ __launch_bounds__(B::kThreads) __attribute__((amdgpu_waves_per_eu(B::kWavesPerEU))) void tree_kernel(TreeArgs a) {
@@ -711,7 +748,7 @@ __global__ __launch_bounds__(B::kThreads) __attribute__((amdgpu_waves_per_eu(B::
     const int64_t T = a.Hkv * S[a.N];
     const int shares = (int)min(T, (int64_t)(a.nwg / team)), used = shares * team;
     if ((int)blockIdx.x >= used) {
-        if (!B::kMass && threadIdx.x == 0) a.cuts[blockIdx.x] = TreeCut{};
+        if (!B::kMass && threadIdx.x == 0) a.rounds[blockIdx.x] = 0;
         return;
     }
     // Work-groups go to the 8 XCDs in turn: neighbours, which may read the same keys for
@@ -721,6 +758,10 @@ __global__ __launch_bounds__(B::kThreads) __attribute__((amdgpu_waves_per_eu(B::
     const int share = w / team, member = w - share * team;
     const int64_t r0 = share_begin(share, T, shares), r1 = share_begin(share + 1, T, shares);
     const int G = a.Hq / a.Hkv;
+    // Beyond three quarters of the last-level cache K and V are streamed, where no other column
+    // block and no other sequence (a cached prefix) reads them again; as in the plain decode.
+    const int64_t tiles = a.Hkv * (B::kTeams ? sT : sP)[a.N];
+    const bool big = B::kStreams && tiles * (kTreeTile * 2 * B::D * (int64_t)sizeof(typename B::T)) > kTreeStreamBytes;
     TreeCut cut = {};
     for (int64_t p = r0; p < r1;) {
         TreeSeg sg;
@@ -735,6 +776,8 @@ __global__ __launch_bounds__(B::kThreads) __attribute__((amdgpu_waves_per_eu(B::
         sg.t1 = (int)(stop - u.begin);
         sg.direct = p == u.begin && stop == end;
         sg.slot = 2 * w + (p == r0 ? 0 : 1);
+        sg.stream = false;
+        if (big) sg.stream = sg.s.P * G <= B::kCols && !shared_page(a, sg.n, (sg.t0 + sg.t1) / 2 * (kTreeTile / kPage));
         if (sg.c0 < sg.cols) {   // (uniform; a team's member may have no block of this sequence)
             if (p == u.begin && stop < end)
                 cut = TreeCut{sg.s.q0, sg.cols, sg.c0, sg.kvh, sg.slot, (int)(wg_of(end - 1, T, shares) - share) + 1, team};
@@ -742,120 +785,147 @@ __global__ __launch_bounds__(B::kThreads) __attribute__((amdgpu_waves_per_eu(B::
         }
         p = stop;
     }
-    if (!B::kMass && threadIdx.x == 0) a.cuts[w] = cut;
+    if (!B::kMass && threadIdx.x == 0) {
+        const int width = join_width<join_lanes(B::D)>(cut.parts);   // a power of two
+        a.rounds[w] = cut.parts > 0 ? (min(B::kCols, cut.cols - cut.c0) + width - 1) >> (31 - __builtin_clz(width)) : 0;
+        a.cuts[w] = cut;
+    }
 }
 
 // Slot of part j of a cut unit that begins in work-group w.
 __device__ inline int part_slot(int w, int first_slot, int step, int j) { return j == 0 ? first_slot : 2 * (w + j * step); }
 
-// Log-sum-exp join of a cut unit's parts, columns first, first + stride .. by one
-// work-group: LR lanes hold a row, 16 bytes each, and as many rows as the work-group
-// has lanes for are read at once, of one column's parts first.  (A wave per
-// column with its parts one after the other: 54 us for 8 units of 64 columns of 64
-// parts, more than the 17 us of the kernel that wrote them.)  out_row(c): the
-// output row of column c.
 struct JoinSmem {
     mf32x4 o[256];
     float ml[64][2];   // (max, sum) per row
 };
 
+// Columns c0 .. c0 + join_width - 1 (those below `here`); out_row(c): the output row.
 template <typename T, int LR, class OutRow>
-__device__ inline void join_columns(const TreeArgs& a, JoinSmem& sm, int cols, int w, const TreeCut& u, int first, int stride,
+__device__ inline void join_columns(const TreeArgs& a, JoinSmem& sm, int cols, int w, const TreeCut& u, int c0, int here,
                                     OutRow out_row) {
-    constexpr int RW = 256 / LR;   // rows at once
-    constexpr int kBatch = 4;      // rows in flight per lane
     const int r = threadIdx.x / LR, l = threadIdx.x % LR;
-    int sp = 1;                    // rows of one column: a lane takes kBatch of its parts at once
-    while (sp * kBatch < u.parts && sp < RW) sp *= 2;
-    const int cpw = RW / sp, sub = r % sp;
-    const int here = min(cols, u.cols - u.c0);
+    const int sp = part_groups<LR>(u.parts), sub = r % sp;
     const bool lane_on = 4 * l < a.D;
-    for (int c0 = first * cpw; c0 < here; c0 += stride * cpw) {   // uniform
-        const int c = c0 + r / sp;
-        float M = -INFINITY, sum = 0.0f;
-        mf32x4 o = {0.f, 0.f, 0.f, 0.f};
-        if (c < here) {
-            for (int j0 = sub; j0 < u.parts; j0 += kBatch * sp) {
-                float lv[kBatch];
-                mf32x4 pv[kBatch];
+    const int c = c0 + r / sp;
+    float M = -INFINITY, sum = 0.0f;
+    mf32x4 o = {0.f, 0.f, 0.f, 0.f};
+    if (c < here) {
+        for (int j0 = sub; j0 < u.parts; j0 += kBatch * sp) {
+            float lv[kBatch];
+            mf32x4 pv[kBatch];
 #pragma unroll
-                for (int b = 0; b < kBatch; ++b) {
-                    const int j = j0 + b * sp;
-                    const bool ok = j < u.parts;
-                    const int64_t row = (int64_t)part_slot(w, u.slot, u.step, ok ? j : j0) * cols + c;
-                    lv[b] = ok ? a.part_lse[row] : -INFINITY;
-                    pv[b] = *reinterpret_cast<const mf32x4*>(a.part_o + row * a.D + (lane_on ? 4 * l : 0));
-                }
-                float mb = M;
-#pragma unroll
-                for (int b = 0; b < kBatch; ++b) mb = fmaxf(mb, lv[b]);
-                if (mb == -INFINITY) continue;   // no key seen so far
-                const float sc = fast_exp2(M - mb);
-                sum *= sc;
-                o *= sc;
-#pragma unroll
-                for (int b = 0; b < kBatch; ++b) {
-                    const float f = fast_exp2(lv[b] - mb);
-                    sum += f;
-                    o += f * pv[b];
-                }
-                M = mb;
+            for (int b = 0; b < kBatch; ++b) {
+                const int j = j0 + b * sp;
+                const bool ok = j < u.parts;
+                const int64_t row = (int64_t)part_slot(w, u.slot, u.step, ok ? j : j0) * cols + c;
+                lv[b] = ok ? a.part_lse[row] : -INFINITY;
+                pv[b] = *reinterpret_cast<const mf32x4*>(a.part_o + row * a.D + (lane_on ? 4 * l : 0));
             }
+            float mb = M;
+#pragma unroll
+            for (int b = 0; b < kBatch; ++b) mb = fmaxf(mb, lv[b]);
+            if (mb == -INFINITY) continue;   // no key seen so far
+            const float sc = fast_exp2(M - mb);
+            sum *= sc;
+            o *= sc;
+#pragma unroll
+            for (int b = 0; b < kBatch; ++b) {
+                const float f = fast_exp2(lv[b] - mb);
+                sum += f;
+                o += f * pv[b];
+            }
+            M = mb;
         }
-        if (sp > 1) {   // uniform
-            sm.o[threadIdx.x] = o;
-            if (l == 0) {
-                sm.ml[r][0] = M;
-                sm.ml[r][1] = sum;
-            }
-            __syncthreads();
-            if (sub == 0) {
-                float top = M;
-                for (int i = 1; i < sp; ++i) top = fmaxf(top, sm.ml[r + i][0]);
-                if (top > -INFINITY) {
-                    float f = fast_exp2(M - top);
-                    sum *= f;
-                    o *= f;
-                    for (int i = 1; i < sp; ++i) {
-                        f = fast_exp2(sm.ml[r + i][0] - top);
-                        sum = fmaf(f, sm.ml[r + i][1], sum);
-                        o += f * sm.o[threadIdx.x + i * LR];
-                    }
+    }
+    if (sp > 1) {   // uniform
+        sm.o[threadIdx.x] = o;
+        if (l == 0) {
+            sm.ml[r][0] = M;
+            sm.ml[r][1] = sum;
+        }
+        __syncthreads();
+        if (sub == 0) {
+            float top = M;
+            for (int i = 1; i < sp; ++i) top = fmaxf(top, sm.ml[r + i][0]);
+            if (top > -INFINITY) {
+                float f = fast_exp2(M - top);
+                sum *= f;
+                o *= f;
+                for (int i = 1; i < sp; ++i) {
+                    f = fast_exp2(sm.ml[r + i][0] - top);
+                    sum = fmaf(f, sm.ml[r + i][1], sum);
+                    o += f * sm.o[threadIdx.x + i * LR];
                 }
             }
-            __syncthreads();
         }
-        if (sub == 0 && c < here && lane_on) {
-            o *= sum == 0.0f ? 0.0f : 1.0f / sum;
-            T* out = out_row(c) + 4 * l;
-            if constexpr (sizeof(T) == 4) *reinterpret_cast<mf32x4*>(out) = o;
-            else *reinterpret_cast<mu32x2*>(out) = mu32x2{pack_pair<T>(o[0], o[1]), pack_pair<T>(o[2], o[3])};
-        }
+        __syncthreads();
+    }
+    if (sub == 0 && c < here && lane_on) {
+        o *= sum == 0.0f ? 0.0f : 1.0f / sum;
+        T* out = out_row(c) + 4 * l;
+        if constexpr (sizeof(T) == 4) *reinterpret_cast<mf32x4*>(out) = o;
+        else *reinterpret_cast<mu32x2*>(out) = mu32x2{pack_pair<T>(o[0], o[1]), pack_pair<T>(o[2], o[3])};
     }
 }
 
-// Grid (work-groups of the first kernel, slices of the columns).
+// The cut units' columns shared by the whole grid: every work-group sums up the
+// rounds of join_columns that the units take and runs rounds blockIdx.x,
+// + gridDim.x ..  (With work-groups tied to the units, a few long units were joined
+// by a few work-groups.)
+constexpr int kMostShares = 2048;   // work-groups of the first kernel
 
 template <typename T, int LR>
 __global__ __launch_bounds__(256) void tree_join_kernel(TreeArgs a, int cols) {
     __shared__ JoinSmem sm;
-    const TreeCut u = a.cuts[blockIdx.x];
-    if (u.parts == 0) return;
-    const int G = a.Hq / a.Hkv;
-    join_columns<T, LR>(a, sm, cols, blockIdx.x, u, blockIdx.y, gridDim.y, [&](int c) {
-        const int col = u.c0 + c, node = col / G;
-        return reinterpret_cast<T*>(a.out) + ((int64_t)(u.q0 + node) * a.Hq + u.kvh * G + (col - node * G)) * a.D;
-    });
+    __shared__ int start[kMostShares + 1];   // rounds before unit w
+    __shared__ int wave_total[4];
+    const int tid = threadIdx.x, lane = tid & 63, wv = tid >> 6;
+    constexpr int kPer = kMostShares / 256;
+    int mine[kPer], sum = 0;   // of units kPer tid ..
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) {
+        mine[i] = kPer * tid + i < a.nwg ? a.rounds[kPer * tid + i] : 0;
+        sum += mine[i];
+    }
+    const int incl = wave_incl_scan(sum);
+    if (lane == 63) wave_total[wv] = incl;
+    __syncthreads();
+    int run = incl - sum;
+    for (int i = 0; i < wv; ++i) run += wave_total[i];
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) {
+        start[kPer * tid + i] = run;
+        run += mine[i];
+    }
+    if (tid == 255) start[kMostShares] = run;
+    __syncthreads();
+    const int rounds = start[kMostShares], G = a.Hq / a.Hkv;
+    for (int x = blockIdx.x; x < rounds; x += gridDim.x) {
+        int lo = 0, hi = kMostShares;   // start[lo] <= x < start[hi]
+        while (hi - lo > 1) {
+            const int mid = (lo + hi) >> 1;
+            if (start[mid] <= x) lo = mid;
+            else hi = mid;
+        }
+        const int w = __builtin_amdgcn_readfirstlane(lo);
+        const TreeCut u = a.cuts[w];
+        join_columns<T, LR>(a, sm, cols, w, u, (x - start[w]) * join_width<LR>(u.parts), min(cols, u.cols - u.c0), [&](int c) {
+            const int col = u.c0 + c, node = col / G;
+            return reinterpret_cast<T*>(a.out) + ((int64_t)(u.q0 + node) * a.Hq + u.kvh * G + (col - node * G)) * a.D;
+        });
+    }
 }
 
-// Kept weights: grid (1 + key blocks of kMassKeys, Hkv, N).  Block 0 joins the
-// output rows of a cut unit.  The others take the unit's log2-sum-exp2 per query
+// Kept weights: grid (kMassJoins + key blocks of kMassKeys, Hkv, N).  The first blocks
+// join the output rows of a cut unit.  The others take the unit's log2-sum-exp2 per query
 // head (of a cut unit, from its parts) and add
 // sum over the group's heads of 2^(score - lse) to their keys' totals, four keys
 // per thread; the first heads' scores are loaded before the log-sum-exps are known.
 constexpr int kMassKeys = 1024;
 constexpr int kMassGroup = 64;   // query heads of a kv head, at most
 constexpr int kMassAhead = 8;    // heads whose scores are in flight
+constexpr int kMassJoins = 2;
 
 template <typename T, int LR>
 __global__ __launch_bounds__(256) void mass_join_kernel(TreeArgs a, int cols) {
@@ -863,7 +933,7 @@ __global__ __launch_bounds__(256) void mass_join_kernel(TreeArgs a, int cols) {
     __shared__ float lse[kMassGroup];
     const int n = blockIdx.z, kvh = blockIdx.y, G = a.Hq / a.Hkv;
     const TreeSeq s = tree_seq(a, n);
-    const int first = ((int)blockIdx.x - 1) * kMassKeys;
+    const int first = ((int)blockIdx.x - kMassJoins) * kMassKeys;
     if (first >= s.L) return;
     const int lane = threadIdx.x & 63, wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int j0 = first + 4 * (int)threadIdx.x;
@@ -890,8 +960,9 @@ __global__ __launch_bounds__(256) void mass_join_kernel(TreeArgs a, int cols) {
     const int w = (int)wg_of(begin, T_, nwg), parts = (int)wg_of(end - 1, T_, nwg) - w + 1;
     const TreeCut u{n, G, 0, kvh, 2 * w + (begin == share_begin(w, T_, nwg) ? 0 : 1), parts, 1};
     if (!keys) {
-        if (parts > 1)
-            join_columns<T, LR>(a, sm, cols, w, u, 0, 1, [&](int c) {
+        const int width = join_width<LR>(parts);
+        for (int c0 = blockIdx.x * width; c0 < G && parts > 1; c0 += kMassJoins * width)
+            join_columns<T, LR>(a, sm, cols, w, u, c0, G, [&](int c) {
                 return reinterpret_cast<T*>(a.out) + ((int64_t)n * a.Hq + kvh * G + c) * a.D;
             });
         return;
@@ -1094,21 +1165,31 @@ TreeChoice choose_f32(int64_t cols, int64_t tiles, bool mass) {
             if (cols <= 32) return choice<FewCols<D, 2, true>>();
         return TreeChoice();
     }
-    // 16 columns also where wider units would not fill the GPU
-    if (D == 256 || cols <= 16 || tiles * ((cols + 63) / 64) < device_cus() / 2) return choice<FewCols<D, 1, false>>();
-    if constexpr (D == 64)
-        if (cols > 32) return choice<FewCols<D, 4, false>>();
-    if constexpr (D < 256) return choice<FewCols<D, 2, false>>();
-    return TreeChoice();
+    // Two tiles of columns where there are tiles for 16 a compute unit (32/8/128, 16 x 2000
+    // keys, 64 columns: 105 us, 112 by single ones); below that single ones (14/2/64, 64 x
+    // 1000, 28 columns: 37 us and 46).
+    if constexpr (D < 256)
+        if (cols > 16 && tiles >= 16 * device_cus()) return choice<FewCols<D, 2, false>>();
+    return choice<FewCols<D, 1, false>>();
 }
 
+// 16-bit pools.  From 129 columns on, units of 256 where there are tiles for 16 a
+// compute unit and most of the last unit is columns (32/8/128, 16 x 4500 keys, 64
+// nodes: 95 us, 113 by units of 64; 1000 tiles: 53 us and 39), else units of 64.  Up to
+// 128 one unit of 128 with eight waves and four tiles in flight (32 columns of 128 dims
+// 56 us, 59 by units of 64 on four waves); at head_dim 256 from 65 columns on (61 x
+// 1100 keys, 16 columns: 93 us, 84 by units of 64).
 template <typename T, int D>
-TreeChoice choose_16(int64_t cols, int64_t, bool mass) {
+TreeChoice choose_16(int64_t cols, int64_t tiles, bool mass) {
     if (mass) return choice<ManyCols<T, D, 1, 8, 4, true>>();
-    if constexpr (D <= 128)
-        if (cols > 128) return choice<ManyCols<T, D, 2, 8, 4>>();
-    if (cols > 64) return choice<ManyCols<T, D, 1, 8, 4>>();
-    return choice<ManyCols<T, D, 1, 4, 2>>();
+    if constexpr (D <= 128) {
+        if (cols <= 128) return choice<ManyCols<T, D, 1, 8, 4>>();
+        if (tiles >= 16 * device_cus() && (cols - 1) % 256 >= 192) return choice<ManyCols<T, D, 2, 8, 4>>();
+        return choice<ManyCols<T, D, 1, 4, 2>>();
+    } else {
+        if (cols <= 64) return choice<ManyCols<T, D, 1, 4, 2>>();
+        return choice<ManyCols<T, D, 1, 8, 4>>();
+    }
 }
 
 template <typename T, int D>
@@ -1134,10 +1215,12 @@ TreeChoice choose(int dtype, int D, int64_t cols, int64_t tiles, bool mass) {
 template <typename T, int LR>
 void launch_join(const TreeArgs& a, int cols, bool mass, hipStream_t st) {
     if (mass) {
-        const dim3 grid((unsigned)(1 + (a.max_len + kMassKeys - 1) / kMassKeys), a.Hkv, a.N);
+        const dim3 grid((unsigned)(kMassJoins + (a.max_len + kMassKeys - 1) / kMassKeys), a.Hkv, a.N);
         mass_join_kernel<T, LR><<<grid, 256, 0, st>>>(a, cols);
     } else {
-        tree_join_kernel<T, LR><<<dim3(a.nwg, cols / 8), 256, 0, st>>>(a, cols);
+        // at most a round for each column of each work-group's one cut unit
+        const int grid = (int)std::min<int64_t>((int64_t)a.nwg * cols, 1024);
+        tree_join_kernel<T, LR><<<grid, 256, 0, st>>>(a, cols);
     }
 }
 
@@ -1156,7 +1239,7 @@ struct TreePlan {
     TreeKernel fn = nullptr;
     int cols = 0, threads = 0, nwg = 0;
     int64_t score_stride = 0;
-    size_t plan = 0, lse = 0, part_lse = 0, part_o = 0, scores = 0, total = 0;
+    size_t rounds = 0, plan = 0, lse = 0, part_lse = 0, part_o = 0, scores = 0, total = 0;
 };
 
 TreePlan make_plan(int N, int rows_most, int Hq, int Hkv, int D, int bs, int max_len, int dtype, bool mass) {
@@ -1172,8 +1255,9 @@ TreePlan make_plan(int N, int rows_most, int Hq, int Hkv, int D, int bs, int max
         p.threads = c.threads;
         const int64_t blocks = (cols + c.cols - 1) / c.cols;
         const int64_t all = (int64_t)n1 * Hkv * blocks * tiles;
-        p.nwg = (int)std::max<int64_t>(1, std::min<int64_t>(resident_workgroups((const void*)c.fn, c.threads), all));
-        p.plan = up256((size_t)p.nwg * sizeof(TreeCut));
+        p.nwg = (int)std::max<int64_t>(1, std::min<int64_t>(std::min(resident_workgroups((const void*)c.fn, c.threads), kMostShares), all));
+        p.rounds = up256((size_t)p.nwg * sizeof(TreeCut));
+        p.plan = p.rounds + up256((size_t)p.nwg * sizeof(int));
         p.lse = p.plan + up256((size_t)(n1 + 1) * sizeof(int64_t));
         p.part_lse = p.lse + (mass ? up256((size_t)n1 * Hq * 4) : 0);
         p.part_o = p.part_lse + up256((size_t)2 * p.nwg * p.cols * 4);
@@ -1231,6 +1315,7 @@ int run_tree(const char* fn, const TreeArgs& all, int rows, int rows_most, int m
         }
         a.nwg = p.nwg;
         a.cuts = reinterpret_cast<TreeCut*>(ws);
+        a.rounds = reinterpret_cast<int*>(ws + p.rounds);
         a.plan = reinterpret_cast<int64_t*>(ws + p.plan);
         a.lse = reinterpret_cast<float*>(ws + p.lse);
         a.part_lse = reinterpret_cast<float*>(ws + p.part_lse);

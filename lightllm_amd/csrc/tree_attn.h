@@ -51,6 +51,7 @@ struct TreeArgs {
     int max_len;          // keys beyond are cut off (the caller's bound)
     int nwg;
     TreeCut* cuts;        // [nwg]
+    int* rounds;          // [nwg]: joining rounds of each work-group's cut unit, 0 without one
     int64_t* plan;        // [N + 1] prefix sums of column blocks x tiles (kept weights alone)
     float* part_o;        // [2 * nwg][kCols][D]
     float* part_lse;      // [2 * nwg][kCols]
@@ -97,7 +98,7 @@ __device__ inline int tree_blocks(const TreeSeq& s, int G) {
 struct TreeSeg {
     TreeSeq s;
     int n, kvh, cols, c0, t0, t1, slot;
-    bool direct;
+    bool direct, stream;   // written out directly; K and V by streaming loads
 };
 
 __device__ inline int64_t wave_incl_scan64(int64_t v) {

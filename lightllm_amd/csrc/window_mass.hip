@@ -17,11 +17,10 @@
 
 #include "attn_common.h"
 #include "decode_mfma.h"
+#include "lds_dma.h"
 
 namespace llkv {
 namespace {
-
-constexpr int kWaves = 4;
 
 struct WindowArgs {
     const void* q;
@@ -31,7 +30,7 @@ struct WindowArgs {
     const int* lens;
     int max_blocks, N, Hq, Hkv, D, bs, max_len;
     float scale_log2;
-    int nblk;          // key blocks of a sequence (by the bound)
+    int nblk;          // key blocks of a sequence, a wave's keys each (by the bound)
     float* part;       // [rows * Hq][nblk] log2-sum-exp2 per key block
     float* lse;        // [rows * Hq]
     float* mass;
@@ -56,37 +55,74 @@ __device__ inline WindowSeq window_seq(const WindowArgs& a, int n) {
 template <typename T>
 constexpr int key_tiles() { return Elem<T>::kDtype == LLKV_DTYPE_F32 ? 2 : 4; }
 template <typename T>
-constexpr int block_keys() { return kWaves * 16 * key_tiles<T>(); }
+constexpr int wave_keys() { return 16 * key_tiles<T>(); }
 
-// SUM false: part[column][block] = the block's log2-sum-exp2 of each column.
+// Columns per LDS chunk: 16 KB of rows (24 KB at head_dim 96, where a chunk has to be
+// whole loads of a work-group).
+template <typename T, int D>
+constexpr int chunk_cols() { return D == 96 ? 512 / (int)sizeof(T) / 2 : 16384 / (D * (int)sizeof(T)); }
+
+// SUM false: part[column][wave] = the log2-sum-exp2 of each column over a wave's keys.
 // SUM true: the totals, from the columns' log2-sum-exp2.
-// Grid (nblk, Hkv, N).
-template <typename T, int D, bool SUM>
-__global__ __launch_bounds__(256) void window_kernel(WindowArgs a) {
+// Grid (nblk / W, Hkv, N), W waves.  The columns' rows go through LDS by direct loads,
+// a ring of three chunks that all waves read: read by each wave from the caches, they
+// took 6 TB/s from L2 and set the time (28/4/128 bf16, 2 x 30001 keys, 64 rows: 72 and
+// 100 us the two passes).  A row's 16-byte units are XOR-ed with the column (rotated by
+// it at head_dim 96), so that the 16 columns of an operand lie in different banks.
+template <typename T, int D, int W, bool SUM>
+__global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(D == 256 ? 1 : 2)))
+void window_kernel(WindowArgs a) {
     using Ops = ScoreOps<T, D>;
     constexpr int KT = key_tiles<T>();
-    __shared__ float ml[2][kWaves][16][2];   // SUM false: the waves' (max, sum) of a column tile
+    constexpr bool k16 = Elem<T>::kDtype != LLKV_DTYPE_F32;
+    constexpr int NC = chunk_cols<T, D>(), CPR = D * (int)sizeof(T) / 16, R = 3;
+    constexpr int LPW = NC * CPR / (64 * W);   // loads of a lane per chunk
+    static_assert(NC % 16 == 0 && NC * CPR % (64 * W) == 0, "chunks are whole loads");
+    __shared__ mu32x4 rows[R][NC * CPR];
     const int n = blockIdx.z, kvh = blockIdx.y;
     const WindowSeq s = window_seq(a, n);
-    const int k0 = blockIdx.x * block_keys<T>();
-    if (k0 >= s.L || s.P == 0) return;
-    const int lane = threadIdx.x & 63, g = lane >> 4, c = lane & 15;
-    const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int G = a.Hq / a.Hkv, cols = s.P * G;
+    if ((int)blockIdx.x * W * wave_keys<T>() >= s.L || s.P == 0) return;   // uniform over the work-group
+    const int tid = threadIdx.x, lane = tid & 63, g = lane >> 4, c = lane & 15;
+    const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int blk = blockIdx.x * W + w;
+    const int k0 = blk * wave_keys<T>();
+    const bool idle = k0 >= s.L;   // the wave has no key: it loads and waits only
+    const int G = a.Hq / a.Hkv, cols = s.P * G, chunks = (cols + NC - 1) / NC;
     const int64_t row_elems = (int64_t)a.Hkv * D;
-    const int* bt = a.bt + (int64_t)n * a.max_blocks;
-    const int npages = (s.L + kPage - 1) / kPage;
+
+    auto place = [](int col, int u) { return (CPR & (CPR - 1)) == 0 ? u ^ (col & (CPR - 1)) : (u + col) % CPR; };
+    auto unit_at = [](int col, int pl) {
+        return (CPR & (CPR - 1)) == 0 ? pl ^ (col & (CPR - 1)) : (pl + CPR * NC - col) % CPR;
+    };
+    const char* const qbase = reinterpret_cast<const char*>(a.q) + ((int64_t)s.q0 * a.Hq + kvh * G) * D * (int)sizeof(T);
+    uint32_t lds[LPW];
+#pragma unroll
+    for (int i = 0; i < LPW; ++i) lds[i] = lds_addr(&rows[0][64 * (LPW * w + i)]);
+    auto load_chunk = [&](int ch) {
+#pragma unroll
+        for (int i = 0; i < LPW; ++i) {
+            const int x = 64 * (LPW * w + i) + lane, r = x / CPR;
+            const int col = min(ch * NC + r, cols - 1), node = col / G;   // (beyond the last: not used)
+            const int64_t off = ((int64_t)node * a.Hq + (col - node * G)) * D * (int)sizeof(T) + unit_at(r, x % CPR) * 16;
+            dma16(qbase + off, lds[i] + (uint32_t)(ch % R) * (NC * CPR * 16));
+        }
+    };
+    load_chunk(0);
+    if (chunks > 1) load_chunk(1);
 
     typename Ops::KReg kr[KT][Ops::NK];
-    int p0[KT];   // the tile's first position
+    if (!idle) {
+        const int* bt = a.bt + (int64_t)n * a.max_blocks;
+        const int last_page = (s.L - 1) / kPage;
 #pragma unroll
-    for (int kt = 0; kt < KT; ++kt) {
-        p0[kt] = k0 + (w * KT + kt) * kPage;
-        const int64_t phys = max(bt[min(p0[kt] / kPage, npages - 1)], 0);   // (beyond the last page: masked)
-        Ops::template load_k<false>(reinterpret_cast<const T*>(a.k) + (int64_t)kvh * D + (phys * kPage + c) * row_elems,
-                                    g, kr[kt]);
+        for (int kt = 0; kt < KT; ++kt) {
+            const int64_t phys = max(bt[min(k0 / kPage + kt, last_page)], 0);   // (beyond the last page: masked)
+            Ops::template load_k<false>(reinterpret_cast<const T*>(a.k) + (int64_t)kvh * D + (phys * kPage + c) * row_elems,
+                                        g, kr[kt]);
+        }
     }
-    const bool whole = p0[KT - 1] + kPage <= s.hist;   // every row sees all of the wave's keys (uniform)
+    const bool whole = k0 + wave_keys<T>() <= s.hist;   // every row sees all of the wave's keys (uniform)
+    const float scale = k16 ? a.scale_log2 : 1.0f;      // 16-bit scores are scaled here, fp32 ones by their Q
 
     float sum[KT][4];
 #pragma unroll
@@ -94,71 +130,90 @@ __global__ __launch_bounds__(256) void window_kernel(WindowArgs a) {
 #pragma unroll
         for (int i = 0; i < 4; ++i) sum[kt][i] = 0.0f;
 
-    for (int c0 = 0; c0 < cols; c0 += 16) {
-        const int col = c0 + c;
-        const bool valid = col < cols;
-        const int node = valid ? col / G : 0;
-        const int64_t qrow = (int64_t)(s.q0 + node) * a.Hq + kvh * G + (col - node * G);
-        typename Ops::QReg q[Ops::NQ];
-        Ops::load_q(reinterpret_cast<const T*>(a.q) + qrow * D, valid, g, a.scale_log2, q);
-        const int last = valid ? min(s.hist + node, s.L - 1) : -1;   // the last key that the column sees
-        const float lse = SUM && valid ? a.lse[qrow] : INFINITY;
-        mf32x4 x[KT];
+    // Column 16 k + c is row `node` under head `head` of the group; the next 16 columns are
+    // 16 / G rows and 16 % G heads further.
+    const int step_node = 16 / G, step_head = 16 - step_node * G;
+    int node = c / G, head = c - node * G;
+    auto column_at = [&]() { return (int64_t)(s.q0 + node) * a.Hq + kvh * G + head; };
+    float next_lse = INFINITY;
+    if (SUM && c < cols) next_lse = a.lse[column_at()];
+
+    for (int ch = 0; ch < chunks; ++ch) {
+        if (ch + 1 < chunks) __builtin_amdgcn_s_waitcnt(vmcnt_imm(LPW));   // all but the next chunk's loads
+        else __builtin_amdgcn_s_waitcnt(vmcnt_imm(0));
+        lds_barrier();   // the chunk is there for all, and the one before it has been read
+        if (ch + 2 < chunks) load_chunk(ch + 2);
+        if (idle) continue;
+        const mu32x4* const here = rows[ch % R];
+        const int stop = min(NC, cols - ch * NC);
+        for (int c0 = 0; c0 < stop; c0 += 16) {
+            const int col = ch * NC + c0 + c;
+            const int64_t at = column_at();
+            const int last = min(s.hist + node, s.L - 1) - k0 - 4 * g;   // the last key that the column sees
+            const float lse = next_lse;
+            node += step_node;
+            head += step_head;
+            node += head >= G ? 1 : 0;
+            head -= head >= G ? G : 0;
+            if constexpr (SUM) {   // a round ahead
+                next_lse = INFINITY;
+                if (col + 16 < cols) next_lse = a.lse[column_at()];
+            }
+            typename Ops::QReg q[Ops::NQ];
 #pragma unroll
-        for (int kt = 0; kt < KT; ++kt) {
-            x[kt] = Ops::scores(kr[kt], q, a.scale_log2);
+            for (int i = 0; i < CPR / 4; ++i) {
+                const mu32x4 x = here[(c0 + c) * CPR + place(c0 + c, 4 * i + g)];
+                if constexpr (k16) {
+                    q[i] = x;
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) q[4 * i + e] = __uint_as_float(x[e]) * a.scale_log2;
+                }
+            }
+            mf32x4 x[KT];
+#pragma unroll
+            for (int kt = 0; kt < KT; ++kt) x[kt] = Ops::scores(kr[kt], q, 1.0f);
             if (!whole) {
 #pragma unroll
-                for (int i = 0; i < 4; ++i)
-                    if (p0[kt] + 4 * g + i > last) x[kt][i] = -INFINITY;
+                for (int kt = 0; kt < KT; ++kt)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) x[kt][i] = 16 * kt + i <= last ? x[kt][i] * scale : -INFINITY;
             }
-        }
-        if constexpr (SUM) {
+            const float f = whole ? scale : 1.0f;
+            if constexpr (SUM) {
 #pragma unroll
-            for (int kt = 0; kt < KT; ++kt)
+                for (int kt = 0; kt < KT; ++kt)
 #pragma unroll
-                for (int i = 0; i < 4; ++i) sum[kt][i] += fast_exp2(x[kt][i] - lse);
-        } else {
-            float m = -INFINITY;
+                    for (int i = 0; i < 4; ++i) sum[kt][i] += fast_exp2(fmaf(x[kt][i], f, -lse));
+            } else {
+                float m = kNegBig, l = 0.0f;
 #pragma unroll
-            for (int kt = 0; kt < KT; ++kt)
+                for (int kt = 0; kt < KT; ++kt)
 #pragma unroll
-                for (int i = 0; i < 4; ++i) m = fmaxf(m, x[kt][i]);
-            m = fmaxf(m, __shfl_xor(m, 16, 64));
-            m = fmaxf(m, __shfl_xor(m, 32, 64));
-            m = fmaxf(m, kNegBig);
-            float l = 0.0f;
+                    for (int i = 0; i < 4; ++i) m = fmaxf(m, x[kt][i] * f);
 #pragma unroll
-            for (int kt = 0; kt < KT; ++kt)
+                for (int kt = 0; kt < KT; ++kt)
 #pragma unroll
-                for (int i = 0; i < 4; ++i) l += fast_exp2(x[kt][i] - m);
-            l += __shfl_xor(l, 16, 64);
-            l += __shfl_xor(l, 32, 64);
-            const int buf = (c0 >> 4) & 1;   // (read before the next barrier, written again after it)
-            if (g == 0) {
-                ml[buf][w][c][0] = m;
-                ml[buf][w][c][1] = l;
-            }
-            lds_barrier();
-            if (w == 0 && g == 0 && valid) {
-                float M = ml[buf][0][c][0];
-#pragma unroll
-                for (int ww = 1; ww < kWaves; ++ww) M = fmaxf(M, ml[buf][ww][c][0]);
-                float S = 0.0f;
-#pragma unroll
-                for (int ww = 0; ww < kWaves; ++ww) S = fmaf(fast_exp2(ml[buf][ww][c][0] - M), ml[buf][ww][c][1], S);
-                a.part[qrow * a.nblk + blockIdx.x] = S == 0.0f ? -INFINITY : M + fast_log2(S);
+                    for (int i = 0; i < 4; ++i) l += fast_exp2(fmaf(x[kt][i], f, -m));
+                // the four lanes of a column
+                float top = fmaxf(m, __shfl_xor(m, 16, 64));
+                top = fmaxf(top, __shfl_xor(top, 32, 64));
+                l *= fast_exp2(m - top);
+                l += __shfl_xor(l, 16, 64);
+                l += __shfl_xor(l, 32, 64);
+                if (g == 0 && col < cols) a.part[at * a.nblk + blk] = l == 0.0f ? -INFINITY : top + fast_log2(l);
             }
         }
     }
     if constexpr (SUM) {
+        if (idle) return;
         float* mass = a.mass + n * a.mass_bs + kvh * a.mass_hs;
 #pragma unroll
         for (int kt = 0; kt < KT; ++kt)
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 const float t = group_sum<16>(sum[kt][i]);
-                const int pos = p0[kt] + 4 * g + i;
+                const int pos = k0 + 16 * kt + 4 * g + i;
                 if (c == 0 && pos < s.L) mass[pos] += t;
             }
     }
@@ -249,15 +304,23 @@ __global__ __launch_bounds__(256) void window_sum_generic_kernel(WindowArgs a) {
 
 bool tuned_shape(int D, int bs) { return bs == kPage && (D == 64 || D == 96 || D == 128 || D == 256); }
 
-int keys_of(int dtype) { return dtype == LLKV_DTYPE_F32 ? block_keys<float>() : block_keys<_Float16>(); }
+int keys_of(int dtype) { return dtype == LLKV_DTYPE_F32 ? wave_keys<float>() : wave_keys<_Float16>(); }
 
+template <typename T, int D, int W>
+void launch_waves(const WindowArgs& a, int max_q_len, hipStream_t st) {
+    const dim3 grid((a.nblk + W - 1) / W, a.Hkv, a.N);
+    const int lse_wgs = (int)std::min<int64_t>(((int64_t)max_q_len * a.Hq + 3) / 4, 65535);
+    window_kernel<T, D, W, false><<<grid, 64 * W, 0, st>>>(a);
+    window_lse_kernel<<<dim3(lse_wgs, a.N), 256, 0, st>>>(a, wave_keys<T>());
+    window_kernel<T, D, W, true><<<grid, 64 * W, 0, st>>>(a);
+}
+
+// Eight waves share a work-group's rows where that leaves work-groups for every
+// compute unit.
 template <typename T, int D>
 void launch_tuned(const WindowArgs& a, int max_q_len, hipStream_t st) {
-    const dim3 grid(a.nblk, a.Hkv, a.N);
-    const int lse_wgs = (int)std::min<int64_t>(((int64_t)max_q_len * a.Hq + 3) / 4, 65535);
-    window_kernel<T, D, false><<<grid, 256, 0, st>>>(a);
-    window_lse_kernel<<<dim3(lse_wgs, a.N), 256, 0, st>>>(a, block_keys<T>());
-    window_kernel<T, D, true><<<grid, 256, 0, st>>>(a);
+    if ((int64_t)a.nblk * a.Hkv * a.N >= 16ll * device_cus()) launch_waves<T, D, 8>(a, max_q_len, st);
+    else launch_waves<T, D, 4>(a, max_q_len, st);
 }
 
 template <typename T>
