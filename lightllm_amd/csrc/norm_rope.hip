@@ -15,9 +15,7 @@
 // the pool unless k_out asks for them).  A group of LPR lanes holds a head row,
 // two 16-byte units per lane: units l and half / W + l, so that both elements
 // of a pair are in one lane, or two neighbouring units of the unrotated tail.
-// The sum of squares is a DPP reduction over the group.  A wave works on one
-// token, so that a lane's pairs are the same in every row it visits: it computes
-// its W angles once, without LDS or barriers, behind the loads of its rows.
+// The sum of squares is a DPP reduction over the group.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -29,6 +27,7 @@ namespace {
 
 constexpr int kMaxAxes = 4;
 constexpr int kMaxPairs = 128;   // head_dim up to 256
+constexpr int kMostAngles = 512; // of a work-group's tokens
 
 struct NormRopeArgs {
     void* qo;
@@ -83,6 +82,19 @@ __device__ inline void load_positions(const NormRopeArgs& a, int t, int (&p)[kMa
     for (int j = 0; j < kMaxAxes; ++j) p[j] = j < a.axes ? a.pos[(int64_t)j * a.T + t] : 0;
 }
 
+// W consecutive floats from a 16-byte aligned address.
+template <int W>
+__device__ inline void load_floats(const float* p, float* f) {
+#pragma unroll
+    for (int i = 0; i < W; i += 4) {
+        const float4 x = *reinterpret_cast<const float4*>(p + i);
+        f[i] = x.x;
+        f[i + 1] = x.y;
+        f[i + 2] = x.z;
+        f[i + 3] = x.w;
+    }
+}
+
 // Where row r of token t (q rows, then k rows, then v rows) is read and written.
 template <typename T>
 struct Row {
@@ -119,84 +131,94 @@ __device__ inline Row<T> row_of(const NormRopeArgs& a, int t, int r, int64_t slo
     return o;
 }
 
-// 16-byte units.  Grid: T * splits waves, four per work-group; wave (t, s) takes
-// the token's rows [s * NI * RPI, (s + 1) * NI * RPI), RPI = 64 / LPR at a time.
-template <typename T, int LPR, int NI>
-__global__ __launch_bounds__(256) void norm_rope_kernel(NormRopeArgs a, int splits) {
+// 16-byte units.  Grid (groups of tpw tokens, slices of a group's rows): a work-group
+// takes rows [slice, slice + per) of its tokens' tpw * R head rows, 256 / LPR at a
+// time, and the tokens' tpw * half angles from LDS, which its threads compute once
+// while their first rows are on the way.
+template <typename T, int LPR>
+__global__ __launch_bounds__(256) void norm_rope_kernel(NormRopeArgs a, int tpw, int per) {
     constexpr int W = Chunk<T>::VEC;
-    constexpr int RPI = 64 / LPR;
-    const int lane = threadIdx.x & 63;
-    const int wave = blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int t = wave / splits;
-    if (t >= a.T) return;
+    constexpr int RPI = 256 / LPR;   // rows at a time
+    constexpr int NI = 2;            // of them in flight
+    __shared__ alignas(16) float cs[2][kMostAngles];   // cosines, sines [token][pair]
+    const int tid = threadIdx.x, l = tid % LPR;
     const int R = a.Hq + 2 * a.Hkv, NU = a.D / W, hu = a.half / W;
-    const int l = lane % LPR;
-    const int r0 = (wave - t * splits) * NI * RPI + lane / LPR;
+    const int t0 = blockIdx.x * tpw, tokens = min(tpw, a.T - t0);
+    const int r0 = blockIdx.y * per, r1 = min(r0 + per, tokens * R);
     const bool rot = l < hu;
     const int ua = rot ? l : 2 * hu + 2 * (l - hu);
     const int ub = rot ? hu + l : ua + 1;
     const bool va = ua < NU, vb = ub < NU;
-    const int64_t slot = a.slots[t];
-
-    // all loads first
     uint4 xa[NI], xb[NI];
     Row<T> row[NI];
+    int tok[NI];
+    auto load = [&](int r) {
 #pragma unroll
-    for (int i = 0; i < NI; ++i) {
-        const int r = r0 + i * RPI;
-        xa[i] = xb[i] = make_uint4(0, 0, 0, 0);
-        if (r < R) {
-            row[i] = row_of<T>(a, t, r, slot);
-            if (va) xa[i] = *reinterpret_cast<const uint4*>(row[i].src + ua * W);
-            if (vb) xb[i] = *reinterpret_cast<const uint4*>(row[i].src + ub * W);
-        } else {
+        for (int i = 0; i < NI; ++i) {
+            const int x = r + i * RPI + tid / LPR;
+            tok[i] = x < r1 ? x / R : 0;
+            xa[i] = xb[i] = make_uint4(0, 0, 0, 0);
             row[i].dst = row[i].dst2 = nullptr;
             row[i].w = nullptr;
             row[i].rotated = false;
+            if (x < r1) {
+                const int t = t0 + tok[i];
+                row[i] = row_of<T>(a, t, x - tok[i] * R, a.slots[t]);
+                if (va) xa[i] = *reinterpret_cast<const uint4*>(row[i].src + ua * W);
+                if (vb) xb[i] = *reinterpret_cast<const uint4*>(row[i].src + ub * W);
+            }
         }
-    }
-    float c[W], s[W];
-    if (rot) {
+    };
+    load(r0);
+    for (int x = tid; x < tokens * a.half; x += 256) {
+        const int k = x / a.half, i = x - k * a.half;
         int p[kMaxAxes];
-        load_positions(a, t, p);
-        const uint32_t codes = axis_word(a, l * W / 16) >> (2 * (l * W % 16));
-#pragma unroll
-        for (int e = 0; e < W; ++e)
-            angle(pick_pos(p, (codes >> (2 * e)) & 3u), a.freq[l * W + e], c[e], s[e]);
+        load_positions(a, t0 + k, p);
+        angle(pick_pos(p, (axis_word(a, i / 16) >> (2 * (i % 16))) & 3u), a.freq[i], cs[0][x], cs[1][x]);
     }
+    __syncthreads();
+    for (int r = r0; r < r1; r += NI * RPI) {
+        if (r > r0) load(r);
 #pragma unroll
-    for (int i = 0; i < NI; ++i) {
-        if (row[i].dst == nullptr && row[i].dst2 == nullptr) continue;
-        if (row[i].rotated) {
-            float f[2 * W];
-            Chunk<T>::unpack(xa[i], f);
-            Chunk<T>::unpack(xb[i], f + W);
-            if (row[i].w != nullptr) {
-                float ss = 0.0f;
+        for (int i = 0; i < NI; ++i) {
+            if (row[i].dst == nullptr && row[i].dst2 == nullptr) continue;
+            if (row[i].rotated) {
+                float f[2 * W];
+                Chunk<T>::unpack(xa[i], f);
+                Chunk<T>::unpack(xb[i], f + W);
+                if (row[i].w != nullptr) {
+                    float ss = 0.0f;
 #pragma unroll
-                for (int e = 0; e < 2 * W; ++e) ss = fmaf(f[e], f[e], ss);
-                ss = group_sum<LPR>(ss);   // lanes of one group share a row and its branch
-                const float n = 1.0f / sqrtf(ss / (float)a.D + a.eps);
+                    for (int e = 0; e < 2 * W; ++e) ss = fmaf(f[e], f[e], ss);
+                    ss = group_sum<LPR>(ss);   // lanes of one group share a row and its branch
+                    const float n = 1.0f / sqrtf(ss / (float)a.D + a.eps);
+                    float wa[W], wb[W];
+                    load_floats<W>(row[i].w + (va ? ua : 0) * W, wa);
+                    load_floats<W>(row[i].w + (vb ? ub : 0) * W, wb);
 #pragma unroll
-                for (int e = 0; e < W; ++e) {
-                    f[e] *= n * (va ? row[i].w[ua * W + e] : 0.0f);
-                    f[W + e] *= n * (vb ? row[i].w[ub * W + e] : 0.0f);
+                    for (int e = 0; e < W; ++e) {
+                        f[e] *= n * wa[e];
+                        f[W + e] *= n * wb[e];
+                    }
                 }
-            }
-            if (rot) {
+                if (rot) {
+                    float c[W], s[W];
+                    load_floats<W>(&cs[0][tok[i] * a.half + l * W], c);
+                    load_floats<W>(&cs[1][tok[i] * a.half + l * W], s);
 #pragma unroll
-                for (int e = 0; e < W; ++e) rotate_pair(c[e], s[e], f[e], f[W + e]);
+                    for (int e = 0; e < W; ++e) rotate_pair(c[e], s[e], f[e], f[W + e]);
+                }
+                xa[i] = Chunk<T>::pack(f);
+                xb[i] = Chunk<T>::pack(f + W);
             }
-            xa[i] = Chunk<T>::pack(f);
-            xb[i] = Chunk<T>::pack(f + W);
-        }
-        if (row[i].dst != nullptr) {
-            if (va) *reinterpret_cast<uint4*>(row[i].dst + ua * W) = xa[i];
-            if (vb) *reinterpret_cast<uint4*>(row[i].dst + ub * W) = xb[i];
-        }
-        if (row[i].dst2 != nullptr) {
-            if (va) *reinterpret_cast<uint4*>(row[i].dst2 + ua * W) = xa[i];
-            if (vb) *reinterpret_cast<uint4*>(row[i].dst2 + ub * W) = xb[i];
+            if (row[i].dst != nullptr) {
+                if (va) *reinterpret_cast<uint4*>(row[i].dst + ua * W) = xa[i];
+                if (vb) *reinterpret_cast<uint4*>(row[i].dst + ub * W) = xb[i];
+            }
+            if (row[i].dst2 != nullptr) {
+                if (va) *reinterpret_cast<uint4*>(row[i].dst2 + ua * W) = xa[i];
+                if (vb) *reinterpret_cast<uint4*>(row[i].dst2 + ub * W) = xb[i];
+            }
         }
     }
 }
@@ -262,13 +284,17 @@ __global__ __launch_bounds__(256) void norm_rope_generic_kernel(NormRopeArgs a) 
     }
 }
 
+// Few tokens: one per group, its rows spread over work-groups.  Many: up to four (512
+// angles) per work-group, which then compute two angles a thread (28/4/128 bf16 with
+// three axes, 5001 tokens: 40 us with every wave computing its own).
 template <typename T, int LPR>
 void launch_units(const NormRopeArgs& a, hipStream_t st) {
-    constexpr int RPI = 64 / LPR;
-    const int iters = (a.Hq + 2 * a.Hkv + RPI - 1) / RPI;
-    const int splits = (iters + 1) / 2;
-    const int64_t waves = (int64_t)a.T * splits;
-    norm_rope_kernel<T, LPR, 2><<<(unsigned)((waves + 3) / 4), 256, 0, st>>>(a, splits);
+    constexpr int RPI = 256 / LPR;
+    const int R = a.Hq + 2 * a.Hkv;
+    const int most = std::max(1, std::min(4, a.half > 0 ? kMostAngles / a.half : 4));
+    const int tpw = (int)std::max<int64_t>(1, std::min<int64_t>(most, a.T / (4ll * device_cus())));
+    const int per = tpw > 1 ? tpw * R : std::min(R, 2 * RPI);
+    norm_rope_kernel<T, LPR><<<dim3((a.T + tpw - 1) / tpw, (tpw * R + per - 1) / per), 256, 0, st>>>(a, tpw, per);
 }
 
 template <typename T>
@@ -359,7 +385,7 @@ extern "C" int llkv_qk_norm_rope_append(void* q_out, void* k_out, const void* q,
     auto aligned = [&](const void* p, int64_t stride) { return !p || (((uintptr_t)p | (uintptr_t)(stride * es)) & 15) == 0; };
     const bool vec = a.half % W == 0 && head_dim % W == 0 && aligned(q, q_stride) && aligned(k, k_stride) &&
                      aligned(v, v_stride) && aligned(q ? q_out : nullptr, q_out_stride) && aligned(k_out, k_out_stride) &&
-                     aligned(k_pool, 0) && aligned(v_pool, 0);
+                     aligned(k_pool, 0) && aligned(v_pool, 0) && aligned(q_weight, 0) && aligned(k_weight, 0);
     hipStream_t st = (hipStream_t)stream;
     if (dtype == LLKV_DTYPE_F32) return launch<float>(a, vec, st);
     if (dtype == LLKV_DTYPE_F16) return launch<_Float16>(a, vec, st);

@@ -70,7 +70,7 @@ constexpr int chunk_cols() { return D == 96 ? 512 / (int)sizeof(T) / 2 : 16384 /
 // 100 us the two passes).  A row's 16-byte units are XOR-ed with the column (rotated by
 // it at head_dim 96), so that the 16 columns of an operand lie in different banks.
 template <typename T, int D, int W, bool SUM>
-__global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(D == 256 ? 1 : 2)))
+__global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(D == 256 ? (sizeof(T) == 2 ? 2 : 1) : (D == 128 && sizeof(T) == 4 ? 3 : 4))))
 void window_kernel(WindowArgs a) {
     using Ops = ScoreOps<T, D>;
     constexpr int KT = key_tiles<T>();
@@ -122,7 +122,10 @@ void window_kernel(WindowArgs a) {
         }
     }
     const bool whole = k0 + wave_keys<T>() <= s.hist;   // every row sees all of the wave's keys (uniform)
-    const float scale = k16 ? a.scale_log2 : 1.0f;      // 16-bit scores are scaled here, fp32 ones by their Q
+    // 16-bit scores are scaled here, fp32 ones by their Q; under a negative scale they change
+    // sign first, so that the largest stays the largest.
+    const float scale = k16 ? fabsf(a.scale_log2) : 1.0f;
+    const bool negative = k16 && a.scale_log2 < 0.0f;
 
     float sum[KT][4];
 #pragma unroll
@@ -173,13 +176,17 @@ void window_kernel(WindowArgs a) {
             mf32x4 x[KT];
 #pragma unroll
             for (int kt = 0; kt < KT; ++kt) x[kt] = Ops::scores(kr[kt], q, 1.0f);
+            if (negative) {
+#pragma unroll
+                for (int kt = 0; kt < KT; ++kt) x[kt] = -x[kt];
+            }
             if (!whole) {
 #pragma unroll
                 for (int kt = 0; kt < KT; ++kt)
 #pragma unroll
                     for (int i = 0; i < 4; ++i) x[kt][i] = 16 * kt + i <= last ? x[kt][i] * scale : -INFINITY;
             }
-            const float f = whole ? scale : 1.0f;
+            const float f = whole ? scale : 1.0f;   // (a masked score stays what it is under a scale of zero)
             if constexpr (SUM) {
 #pragma unroll
                 for (int kt = 0; kt < KT; ++kt)
@@ -190,7 +197,8 @@ void window_kernel(WindowArgs a) {
 #pragma unroll
                 for (int kt = 0; kt < KT; ++kt)
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) m = fmaxf(m, x[kt][i] * f);
+                    for (int i = 0; i < 4; i += 2) m = fmaxf(fmaxf(m, x[kt][i]), x[kt][i + 1]);
+                m *= f;
 #pragma unroll
                 for (int kt = 0; kt < KT; ++kt)
 #pragma unroll
@@ -319,7 +327,7 @@ void launch_waves(const WindowArgs& a, int max_q_len, hipStream_t st) {
 // compute unit.
 template <typename T, int D>
 void launch_tuned(const WindowArgs& a, int max_q_len, hipStream_t st) {
-    if ((int64_t)a.nblk * a.Hkv * a.N >= 16ll * device_cus()) launch_waves<T, D, 8>(a, max_q_len, st);
+    if ((int64_t)a.nblk * a.Hkv * a.N >= 8ll * device_cus()) launch_waves<T, D, 8>(a, max_q_len, st);
     else launch_waves<T, D, 4>(a, max_q_len, st);
 }
 
