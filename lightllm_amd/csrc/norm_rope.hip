@@ -169,12 +169,29 @@ __global__ __launch_bounds__(256) void norm_rope_kernel(NormRopeArgs a, int tpw,
             }
         }
     };
+    // The angles' positions and frequencies before the rows (loads return in order).
+    constexpr int NA = kMostAngles / 256;
+    int pos[NA];
+    float freq[NA];
+#pragma unroll
+    for (int j = 0; j < NA; ++j) {
+        const int x = tid + 256 * j;
+        pos[j] = 0;
+        freq[j] = 0.0f;
+        if (x < tokens * a.half) {
+            const int k = x / a.half, i = x - k * a.half;
+            const int axis = (int)(axis_word(a, i / 16) >> (2 * (i % 16)) & 3u);
+            pos[j] = a.pos[(int64_t)axis * a.T + t0 + k];
+            freq[j] = a.freq[i];
+        }
+    }
+    __builtin_amdgcn_sched_barrier(0);
     load(r0);
-    for (int x = tid; x < tokens * a.half; x += 256) {
-        const int k = x / a.half, i = x - k * a.half;
-        int p[kMaxAxes];
-        load_positions(a, t0 + k, p);
-        angle(pick_pos(p, (axis_word(a, i / 16) >> (2 * (i % 16))) & 3u), a.freq[i], cs[0][x], cs[1][x]);
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int j = 0; j < NA; ++j) {
+        const int x = tid + 256 * j;
+        if (x < tokens * a.half) angle(pos[j], freq[j], cs[0][x], cs[1][x]);
     }
     __syncthreads();
     for (int r = r0; r < r1; r += NI * RPI) {
