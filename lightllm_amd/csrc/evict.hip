@@ -287,14 +287,20 @@ __global__ __launch_bounds__(kSelThreads) void select_chunk_kernel(SelectArgs a,
         }
         const uint32_t* h = a.hist[p & 1] + base * (kBins / 2) + (kBins / 2 - 1 - tid);
         int hi = 0, lo = 0;
-        for (int i = 0; i < chunks; ++i) {
-            const uint32_t v = h[(int64_t)i * (kBins / 2)];
-            if (i == c) {
-                before_hi = hi;
-                before_lo = lo;
+        constexpr int kAhead = 16;
+        for (int i0 = 0; i0 < chunks; i0 += kAhead) {
+            uint32_t v[kAhead];
+#pragma unroll
+            for (int i = 0; i < kAhead; ++i) v[i] = i0 + i < chunks ? h[(int64_t)(i0 + i) * (kBins / 2)] : 0u;
+#pragma unroll
+            for (int i = 0; i < kAhead; ++i) {
+                if (i0 + i == c) {
+                    before_hi = hi;
+                    before_lo = lo;
+                }
+                lo += (int)(v[i] & 0xFFFFu);
+                hi += (int)(v[i] >> 16);
             }
-            lo += (int)(v & 0xFFFFu);
-            hi += (int)(v >> 16);
         }
         find_digit(s, hi, lo, left, digit, left);
         const uint32_t above = prefix;
@@ -350,45 +356,38 @@ __device__ inline int64_t part_at(const CompactArgs& a, const int* table, int bl
     return (page * a.bs + pos % a.bs) * a.row_bytes + h * a.part_bytes;
 }
 
-// Source and destination pages are different: a parallel copy.  Grid (blocks of
-// kept positions, heads, N); a work-group takes 256 / lanes_per_part positions
-// at a time, kCopies of them in flight per lane, K and V.
-constexpr int kCopies = 2;
+// A load of a row that is not read again: past the caches, so that they keep what is
+// written (32 x 1024 rows of 8 x 128 fp16 with its selection 72 us a call, 63 so; with
+// stores past them as well 68).
+template <typename U>
+__device__ inline U load_once(const char* p) {
+    if constexpr (sizeof(U) == 16) {
+        typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
+        return __builtin_bit_cast(U, __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(p)));
+    } else {
+        return *reinterpret_cast<const U*>(p);
+    }
+}
 
+// Source and destination pages are different: a parallel copy.  Grid (blocks of
+// kept positions, heads, N); `lanes` lanes of a work-group take a row part, in K and
+// in V, and nothing more: with two rows a lane, an eighth fewer work-groups in flight
+// behind the chain count -> position -> page -> row (32 x 1024 rows of 8 x 128 fp16
+// 67 us, this 58).
 template <typename U>
 __global__ __launch_bounds__(256) void compact_copy_kernel(CompactArgs a, int lanes) {
     const int n = blockIdx.z, h = blockIdx.y;
-    const int r = threadIdx.x / lanes, u0 = threadIdx.x - r * lanes, rows = 256 / lanes;
-    if (r >= rows) return;
-    const int count = min(a.counts[n], a.M), start = a.start ? a.start[n] : 0;
-    const int* keep = a.keep + ((int64_t)n * a.H + h) * a.M;
-    for (int i0 = blockIdx.x * rows * kCopies; i0 < count; i0 += gridDim.x * rows * kCopies) {
-        int64_t s[kCopies], d[kCopies];
-#pragma unroll
-        for (int e = 0; e < kCopies; ++e) {
-            const int i = i0 + e * rows + r;
-            s[e] = d[e] = -1;
-            if (i < count) {
-                s[e] = part_at(a, a.src, a.src_blocks, n, h, keep[i]);
-                d[e] = part_at(a, a.dst, a.dst_blocks, n, h, start + i);
-            }
-        }
-        for (int u = u0; u < a.units; u += lanes) {
-            const int64_t off = (int64_t)u * sizeof(U);
-            U kk[kCopies], vv[kCopies];
-#pragma unroll
-            for (int e = 0; e < kCopies; ++e)
-                if (s[e] >= 0 && d[e] >= 0) {
-                    kk[e] = *reinterpret_cast<const U*>(a.k + s[e] + off);
-                    vv[e] = *reinterpret_cast<const U*>(a.v + s[e] + off);
-                }
-#pragma unroll
-            for (int e = 0; e < kCopies; ++e)
-                if (s[e] >= 0 && d[e] >= 0) {
-                    *reinterpret_cast<U*>(a.k + d[e] + off) = kk[e];
-                    *reinterpret_cast<U*>(a.v + d[e] + off) = vv[e];
-                }
-        }
+    const int r = threadIdx.x / lanes, rows = 256 / lanes;
+    const int i = blockIdx.x * rows + r;
+    if (i >= min(a.counts[n], a.M)) return;
+    const int64_t s = part_at(a, a.src, a.src_blocks, n, h, a.keep[((int64_t)n * a.H + h) * a.M + i]);
+    const int64_t d = part_at(a, a.dst, a.dst_blocks, n, h, (a.start ? a.start[n] : 0) + i);
+    if (s < 0 || d < 0) return;
+    for (int u = threadIdx.x - r * lanes; u < a.units; u += lanes) {
+        const int64_t off = (int64_t)u * sizeof(U);
+        const U kk = load_once<U>(a.k + s + off), vv = load_once<U>(a.v + s + off);
+        *reinterpret_cast<U*>(a.k + d + off) = kk;
+        *reinterpret_cast<U*>(a.v + d + off) = vv;
     }
 }
 
@@ -399,12 +398,11 @@ __global__ __launch_bounds__(256) void compact_copy_kernel(CompactArgs a, int la
 // round's destinations.  A work-group owns kUnits units of every row of one
 // (sequence, head part) in K or in V, which no other work-group touches.
 // Grid (units / kUnits, H, 2 N).
-constexpr int kUnits = 8;
-constexpr int kRows = 256 / kUnits;
 constexpr int kLoads = 4;
 
-template <typename U>
+template <typename U, int kUnits>
 __global__ __launch_bounds__(256) void compact_inplace_kernel(CompactArgs a) {
+    constexpr int kRows = 256 / kUnits;
     const int n = blockIdx.z >> 1, h = blockIdx.y;
     char* pool = blockIdx.z & 1 ? a.v : a.k;
     const int u = blockIdx.x * kUnits + threadIdx.x % kUnits;
@@ -471,7 +469,7 @@ void launch_compact(CompactArgs a, bool in_place, hipStream_t st) {
     a.units = (int)(a.part_bytes / sizeof(U));
     int lanes = 1;   // of a part: a power of two up to the work-group
     while (lanes < a.units && lanes < 256) lanes *= 2;
-    const int per = 256 / lanes * kCopies;
+    const int per = 256 / lanes;
     constexpr int kMost = 32767;   // sequences per launch (a grid's extent in z)
     const int N = a.N;
     for (int n0 = 0; n0 < N; n0 += kMost) {
@@ -486,7 +484,11 @@ void launch_compact(CompactArgs a, bool in_place, hipStream_t st) {
             compact_copy_kernel<U><<<dim3((a.M + per - 1) / per, a.H, b.N), 256, 0, st>>>(b, lanes);
             continue;
         }
-        compact_inplace_kernel<U><<<dim3((a.units + kUnits - 1) / kUnits, a.H, 2 * b.N), 256, 0, st>>>(b);
+        // a few rows: wide parts of them in one round; many: narrow parts, for work-groups enough
+        const bool few = a.M <= 256 / 64 * kLoads;
+        const dim3 grid((a.units + (few ? 64 : 8) - 1) / (few ? 64 : 8), a.H, 2 * b.N);
+        if (few) compact_inplace_kernel<U, 64><<<grid, 256, 0, st>>>(b);
+        else compact_inplace_kernel<U, 8><<<grid, 256, 0, st>>>(b);
     }
 }
 
@@ -555,6 +557,8 @@ extern "C" int llkv_evict_select(int* keep, int* counts, float* mass_out, int64_
         for (int pass = 0; pass < 4; ++pass) select_chunk_kernel<<<grid, kSelThreads, 0, st>>>(a, pass);
     } else if (max_seq_len <= 4 * kSelThreads) {
         select_kernel<4><<<units, kSelThreads, 0, st>>>(a);
+    } else if (max_seq_len <= 8 * kSelThreads) {
+        select_kernel<8><<<units, kSelThreads, 0, st>>>(a);
     } else {
         select_kernel<kOnePass><<<units, kSelThreads, 0, st>>>(a);
     }
