@@ -334,6 +334,12 @@ __global__ __launch_bounds__(kSelThreads) void select_chunk_kernel(SelectArgs a,
     write_kept<VPT>(a, u, s, k, c * kChunk, prefix, left, ga, ea);
 }
 
+// Units of a move.  (Native vectors: an array of HIP's uint4 went to LDS, addressed by
+// the work-group's size, which is read from the launch packet in host memory: an
+// in-place move of nine rows 17 us.)
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+
 struct CompactArgs {
     char* k;
     char* v;
@@ -348,12 +354,14 @@ struct CompactArgs {
     int64_t part_bytes;  // of a part: row_bytes / H
 };
 
-// Byte offset of head part h of position pos, or -1 where the table has no page.
+// Byte offset of head part h of position pos, or -1 where the table has no page.  No
+// branch around the load, so that several of them are under way at once.
 __device__ inline int64_t part_at(const CompactArgs& a, const int* table, int blocks, int n, int h, int pos) {
-    if (pos < 0 || pos / a.bs >= blocks) return -1;
-    const int64_t page = table[(int64_t)n * blocks + pos / a.bs];
-    if (page < 0) return -1;
-    return (page * a.bs + pos % a.bs) * a.row_bytes + h * a.part_bytes;
+    const int index = max(pos, 0) / a.bs;
+    const bool inside = pos >= 0 && index < blocks;
+    const int64_t page = table[(int64_t)n * blocks + (inside ? index : 0)];
+    const int64_t at = (page * a.bs + (max(pos, 0) - index * a.bs)) * a.row_bytes + h * a.part_bytes;
+    return inside && page >= 0 ? at : -1;
 }
 
 // A load of a row that is not read again: past the caches, so that they keep what is
@@ -362,8 +370,7 @@ __device__ inline int64_t part_at(const CompactArgs& a, const int* table, int bl
 template <typename U>
 __device__ inline U load_once(const char* p) {
     if constexpr (sizeof(U) == 16) {
-        typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
-        return __builtin_bit_cast(U, __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(p)));
+        return __builtin_nontemporal_load(reinterpret_cast<const U*>(p));
     } else {
         return *reinterpret_cast<const U*>(p);
     }
@@ -412,20 +419,21 @@ __global__ __launch_bounds__(256) void compact_inplace_kernel(CompactArgs a) {
     const int* keep = a.keep + ((int64_t)n * a.H + h) * a.M;
     for (int i0 = 0; i0 < count; i0 += kLoads * kRows) {
         U x[kLoads];
-        int64_t to[kLoads];
+        int from[kLoads];
+        int64_t at[kLoads], to[kLoads];
+#pragma unroll
+        for (int e = 0; e < kLoads; ++e) from[e] = keep[min(i0 + e * kRows + r, count - 1)];
 #pragma unroll
         for (int e = 0; e < kLoads; ++e) {
             const int i = i0 + e * kRows + r;
-            to[e] = -1;
-            if (i < count && u < a.units) {
-                const int from = keep[i];
-                const int64_t s = part_at(a, a.src, a.src_blocks, n, h, from);
-                if (s >= 0 && from != start + i) {   // (a row that stays is not touched)
-                    to[e] = part_at(a, a.src, a.src_blocks, n, h, start + i);
-                    x[e] = *reinterpret_cast<const U*>(pool + s + off);
-                }
-            }
+            at[e] = part_at(a, a.src, a.src_blocks, n, h, from[e]);
+            to[e] = part_at(a, a.src, a.src_blocks, n, h, start + i);
+            // (a row that stays is not touched)
+            if (i >= count || u >= a.units || at[e] < 0 || from[e] == start + i) to[e] = -1;
         }
+#pragma unroll
+        for (int e = 0; e < kLoads; ++e)
+            if (to[e] >= 0) x[e] = *reinterpret_cast<const U*>(pool + at[e] + off);
         __atomic_signal_fence(__ATOMIC_SEQ_CST);
         __builtin_amdgcn_s_waitcnt(0x3F70);   // vmcnt(0): this wave's rows have arrived
         __builtin_amdgcn_s_barrier();
@@ -601,8 +609,8 @@ extern "C" int llkv_compact(void* k_pool, void* v_pool, const int* src_table, in
     a.part_bytes = a.row_bytes / keep_heads;
     hipStream_t st = (hipStream_t)stream;
     switch (unit_bytes(a.part_bytes, k_pool, v_pool)) {
-        case 16: launch_compact<uint4>(a, !dst_table, st); break;
-        case 8: launch_compact<uint2>(a, !dst_table, st); break;
+        case 16: launch_compact<u32x4>(a, !dst_table, st); break;
+        case 8: launch_compact<u32x2>(a, !dst_table, st); break;
         case 4: launch_compact<uint32_t>(a, !dst_table, st); break;
         default: launch_compact<uint16_t>(a, !dst_table, st); break;
     }

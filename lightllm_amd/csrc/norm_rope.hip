@@ -251,7 +251,7 @@ __global__ __launch_bounds__(256) void norm_rope_generic_kernel(NormRopeArgs a) 
     if (t >= a.T) return;
     const Row<T> row = row_of<T>(a, t, wave - t * R, a.slots[t]);
     if (row.dst == nullptr && row.dst2 == nullptr) return;
-    T raw[8];     // pair halves (0, 1), (2, 3), then the tail
+    float f[8];   // pair halves (0, 1), (2, 3), then the tail
     int dim[8];
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
@@ -264,40 +264,40 @@ __global__ __launch_bounds__(256) void norm_rope_generic_kernel(NormRopeArgs a) 
         const int d = 2 * a.half + lane + 64 * j;
         dim[4 + j] = d < a.D ? d : -1;
     }
+    if (!row.rotated) {   // a v row: moved bit for bit
 #pragma unroll
-    for (int j = 0; j < 8; ++j)
-        if (dim[j] >= 0) raw[j] = row.src[dim[j]];
-    if (row.rotated) {
-        float f[8], ss = 0.0f;
+        for (int j = 0; j < 8; ++j)
+            if (dim[j] >= 0) row.dst[dim[j]] = row.src[dim[j]];
+        return;
+    }
+    float ss = 0.0f;
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            f[j] = dim[j] >= 0 ? Elem<T>::to_f32(raw[j]) : 0.0f;
-            ss = fmaf(f[j], f[j], ss);
-        }
-        if (row.w != nullptr) {
-            const float n = 1.0f / sqrtf(wave_sum(ss) / (float)a.D + a.eps);
+    for (int j = 0; j < 8; ++j) {
+        f[j] = 0.0f;
+        if (dim[j] >= 0) f[j] = Elem<T>::to_f32(row.src[dim[j]]);
+        ss = fmaf(f[j], f[j], ss);
+    }
+    if (row.w != nullptr) {
+        const float n = 1.0f / sqrtf(wave_sum(ss) / (float)a.D + a.eps);
 #pragma unroll
-            for (int j = 0; j < 8; ++j)
-                if (dim[j] >= 0) f[j] *= n * row.w[dim[j]];
-        }
-        int p[kMaxAxes];
-        if (a.half > 0) load_positions(a, t, p);
+        for (int j = 0; j < 8; ++j)
+            if (dim[j] >= 0) f[j] *= n * row.w[dim[j]];
+    }
+    int p[kMaxAxes];
+    if (a.half > 0) load_positions(a, t, p);
 #pragma unroll
-        for (int j = 0; j < 2; ++j) {
-            const int i = lane + 64 * j;
-            if (i >= a.half) continue;
-            float c, s;
-            angle(pick_pos(p, (axis_word(a, i / 16) >> (2 * (i % 16))) & 3u), a.freq[i], c, s);
-            rotate_pair(c, s, f[2 * j], f[2 * j + 1]);
-        }
-#pragma unroll
-        for (int j = 0; j < 8; ++j) raw[j] = Elem<T>::from_f32(f[j]);
+    for (int j = 0; j < 2; ++j) {
+        const int i = lane + 64 * j;
+        if (i >= a.half) continue;
+        float c, s;
+        angle(pick_pos(p, (axis_word(a, i / 16) >> (2 * (i % 16))) & 3u), a.freq[i], c, s);
+        rotate_pair(c, s, f[2 * j], f[2 * j + 1]);
     }
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
         if (dim[j] < 0) continue;
-        if (row.dst != nullptr) row.dst[dim[j]] = raw[j];
-        if (row.dst2 != nullptr) row.dst2[dim[j]] = raw[j];
+        if (row.dst != nullptr) row.dst[dim[j]] = Elem<T>::from_f32(f[j]);
+        if (row.dst2 != nullptr) row.dst2[dim[j]] = Elem<T>::from_f32(f[j]);
     }
 }
 
