@@ -70,18 +70,6 @@ __device__ inline uint32_t axis_word(const NormRopeArgs& a, int word) {
     return w;
 }
 
-__device__ inline int pick_pos(const int (&p)[kMaxAxes], uint32_t code) {
-    int r = p[0];
-#pragma unroll
-    for (int j = 1; j < kMaxAxes; ++j) r = code == (uint32_t)j ? p[j] : r;
-    return r;
-}
-
-__device__ inline void load_positions(const NormRopeArgs& a, int t, int (&p)[kMaxAxes]) {
-#pragma unroll
-    for (int j = 0; j < kMaxAxes; ++j) p[j] = j < a.axes ? a.pos[(int64_t)j * a.T + t] : 0;
-}
-
 // W consecutive floats from a 16-byte aligned address.
 template <int W>
 __device__ inline void load_floats(const float* p, float* f) {
@@ -283,14 +271,13 @@ __global__ __launch_bounds__(256) void norm_rope_generic_kernel(NormRopeArgs a) 
         for (int j = 0; j < 8; ++j)
             if (dim[j] >= 0) f[j] *= n * row.w[dim[j]];
     }
-    int p[kMaxAxes];
-    if (a.half > 0) load_positions(a, t, p);
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
         const int i = lane + 64 * j;
         if (i >= a.half) continue;
         float c, s;
-        angle(pick_pos(p, (axis_word(a, i / 16) >> (2 * (i % 16))) & 3u), a.freq[i], c, s);
+        const uint32_t axis = (axis_word(a, i / 16) >> (2 * (i % 16))) & 3u;
+        angle(a.pos[(int64_t)axis * a.T + t], a.freq[i], c, s);
         rotate_pair(c, s, f[2 * j], f[2 * j + 1]);
     }
 #pragma unroll
