@@ -150,7 +150,7 @@ int llkv_rope_append(void* q, void* k, const void* v, void* k_pool, void* v_pool
  * q [num_tokens, Hq, D], k and v [num_tokens, Hkv, D]: each token's heads are
  * contiguous and tokens are *_stride elements apart (slices of one fused
  * projection).  q (may be NULL) goes to q_out; k and v rows go to pool row
- * slot_mapping[t] (negative: no pool write) and, with k_out not NULL, the k row
+ * slot_mapping[t] (negative: no pool write; the others distinct) and, with k_out not NULL, the k row
  * to k_out as well.  q_out / k_out may be q / k themselves (same stride);
  * otherwise inputs and outputs must not overlap.
  * positions: device int32 [num_axes, num_tokens]; 1 <= num_axes <= 4.

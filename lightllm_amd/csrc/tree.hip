@@ -2,13 +2,13 @@
 // step that adds its attention weights to each key's total (gfx950).  The
 // schedule is in tree_attn.h.
 //
-// Bodies.  FewCols: a page of 16 keys at a time, K and V straight
+// Bodies.  FewCols (fp32): a page of 16 keys at a time, K and V straight
 // into the operand registers of the matrix instructions in the decode's layouts
 // (decode_mfma.h), NCT tiles of 16 columns against each.  The four waves of a
 // work-group take the four pages of a tile and join their softmax states
-// through LDS at the end of a segment.  ManyCols (16-bit pools, head_dim 64 / 128
-// / 256): tiles of K and V staged in LDS by direct loads, double-buffered, each
-// wave with its own 16 or 32 columns over all keys, as the prefill.
+// through LDS at the end of a segment.  ManyCols (16-bit pools): tiles of K and V
+// staged in a ring in LDS by direct loads, each wave with its own 16 or 32
+// columns over all keys, as the prefill.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -1007,7 +1007,7 @@ __global__ __launch_bounds__(256) void mass_join_kernel(TreeArgs a, int cols) {
 // (row, query head).  MASS: one wave per (sequence, kv head), head after head,
 // the scores kept, then the totals.
 template <typename T, bool MASS>
-__global__ __launch_bounds__(64) void tree_generic_kernel(TreeArgs a, int rows) {
+__global__ __launch_bounds__(64) void tree_generic_kernel(TreeArgs a) {
     __shared__ float q_s[256];
     __shared__ float p_s[64];
     __shared__ int64_t row_s[64];
@@ -1301,16 +1301,15 @@ int run_tree(const char* fn, const TreeArgs& all, int rows, int rows_most, int m
         }
         if (!tuned) {
             const dim3 grid(mass ? a.N : rows, mass ? a.Hkv : a.Hq);
-            const int nrows = rows;
             if (dtype == LLKV_DTYPE_F32)
-                mass ? tree_generic_kernel<float, true><<<grid, 64, 0, st>>>(a, nrows)
-                     : tree_generic_kernel<float, false><<<grid, 64, 0, st>>>(a, nrows);
+                mass ? tree_generic_kernel<float, true><<<grid, 64, 0, st>>>(a)
+                     : tree_generic_kernel<float, false><<<grid, 64, 0, st>>>(a);
             else if (dtype == LLKV_DTYPE_F16)
-                mass ? tree_generic_kernel<_Float16, true><<<grid, 64, 0, st>>>(a, nrows)
-                     : tree_generic_kernel<_Float16, false><<<grid, 64, 0, st>>>(a, nrows);
+                mass ? tree_generic_kernel<_Float16, true><<<grid, 64, 0, st>>>(a)
+                     : tree_generic_kernel<_Float16, false><<<grid, 64, 0, st>>>(a);
             else
-                mass ? tree_generic_kernel<bf16_t, true><<<grid, 64, 0, st>>>(a, nrows)
-                     : tree_generic_kernel<bf16_t, false><<<grid, 64, 0, st>>>(a, nrows);
+                mass ? tree_generic_kernel<bf16_t, true><<<grid, 64, 0, st>>>(a)
+                     : tree_generic_kernel<bf16_t, false><<<grid, 64, 0, st>>>(a);
             continue;
         }
         a.nwg = p.nwg;

@@ -626,13 +626,14 @@ def build_tree(parents: torch.Tensor, cu_q: torch.Tensor, seq_lens: torch.Tensor
     return tree_mask, positions
 
 
+# By the device, too: a launch is as large as the device's compute units hold.
 @functools.lru_cache(maxsize=256)
-def _tree_size(*shape: int) -> int:
+def _tree_size(device: int, *shape: int) -> int:
     return lib().llkv_paged_tree_attention_workspace_size(*shape)
 
 
 @functools.lru_cache(maxsize=256)
-def _mass_size(*shape: int) -> int:
+def _mass_size(device: int, *shape: int) -> int:
     return lib().llkv_paged_decode_mass_workspace_size(*shape)
 
 
@@ -656,10 +657,11 @@ def paged_tree_attention(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Te
     else:
         _check(out, dtype, (tq, hq, d), device, "out")
     max_q_len, max_seq_len, dt = int(max_q_len), int(max_seq_len), dtype_code(dtype)
-    ws, nbytes, held = _scratch(_tree_size(n, max_q_len, hq, hkv, d, bs, max_seq_len, dt), workspace, device, stream)
+    need = _tree_size(device, n, max_q_len, hq, hkv, d, bs, max_seq_len, dt)
+    ws, nbytes, held = _scratch(need, workspace, device, stream)
     check(lib().llkv_paged_tree_attention(_ptr(out), _ptr(q), _ptr(k_pool), _ptr(v_pool), _ptr(block_table),
-                                          blocks, _ptr(cu_q), _ptr(seq_lens), _ptr(tree_mask), words, n, tq, max_q_len, max_seq_len, hq, hkv, d, bs,
-                                          _scale(scale, d), dt, ws, nbytes, _stream(stream)))
+                                          blocks, _ptr(cu_q), _ptr(seq_lens), _ptr(tree_mask), words, n, tq, max_q_len,
+                                          max_seq_len, hq, hkv, d, bs, _scale(scale, d), dt, ws, nbytes, _stream(stream)))
     return out
 
 
@@ -680,9 +682,10 @@ def paged_decode_mass(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tenso
         out = _empty((b, hq, d), dtype, device, stream)
     else:
         _check(out, dtype, (b, hq, d), device, "out")
-    ws, nbytes, held = _scratch(_mass_size(b, hq, hkv, d, bs, max_seq_len, dt), workspace, device, stream)
+    ws, nbytes, held = _scratch(_mass_size(device, b, hq, hkv, d, bs, max_seq_len, dt), workspace, device, stream)
     check(lib().llkv_paged_decode_mass(_ptr(out), _ptr(mass), mass_bs, mass_hs, _ptr(q), _ptr(k_pool), _ptr(v_pool),
-                                       _ptr(block_table), _ptr(seq_lens), b, hq, hkv, d, bs, blocks, max_seq_len, _scale(scale, d), dt, ws, nbytes, _stream(stream)))
+                                       _ptr(block_table), _ptr(seq_lens), b, hq, hkv, d, bs, blocks, max_seq_len,
+                                       _scale(scale, d), dt, ws, nbytes, _stream(stream)))
     return out
 
 
@@ -704,8 +707,8 @@ def paged_window_mass(q: torch.Tensor, k_pool: torch.Tensor, block_table: torch.
     need = lib().llkv_paged_window_mass_workspace_size(tq, hq, max_seq_len, dt)
     ws, nbytes, held = _scratch(need, workspace, device, stream)
     check(lib().llkv_paged_window_mass(_ptr(mass), mass_bs, mass_hs, _ptr(q), _ptr(k_pool), _ptr(block_table),
-                                       blocks, _ptr(cu_q), _ptr(seq_lens), n, tq, max_q_len, max_seq_len, hq, hkv, d, bs, _scale(scale, d), dt, ws, nbytes,
-                                       _stream(stream)))
+                                       blocks, _ptr(cu_q), _ptr(seq_lens), n, tq, max_q_len, max_seq_len, hq, hkv, d, bs,
+                                       _scale(scale, d), dt, ws, nbytes, _stream(stream)))
 
 
 def evict_select(mass: torch.Tensor, seq_lens: torch.Tensor, budget: int, max_seq_len: int, sinks: int = 0,
@@ -722,7 +725,8 @@ def evict_select(mass: torch.Tensor, seq_lens: torch.Tensor, budget: int, max_se
     keep = _empty((n, hkv, budget), torch.int32, device, stream)
     counts = _empty((n,), torch.int32, device, stream)
     out = _empty((n, hkv, width), torch.float32, device, stream)
-    ws, nbytes, held = _scratch(lib().llkv_evict_select_workspace_size(n, hkv, max_seq_len), workspace, device, stream)
+    need = lib().llkv_evict_select_workspace_size(n, hkv, max_seq_len)
+    ws, nbytes, held = _scratch(need, workspace, device, stream)
     check(lib().llkv_evict_select(_ptr(keep), _ptr(counts), _ptr(out), hkv * width, width, width, _ptr(mass), mass_bs,
                                   mass_hs, _ptr(seq_lens), n, hkv, max_seq_len, budget, sinks, recent, ws, nbytes,
                                   _stream(stream)))
