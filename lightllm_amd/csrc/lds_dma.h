@@ -28,7 +28,15 @@ __device__ inline void dma16(const void* gptr, uint32_t la) {
                  : "memory", "m0");
 }
 
-// The same with a wave-uniform base (scalar registers) and a 32-bit per-lane
+// 4 bytes per lane, to lds + 4 L.
+__device__ inline void dma4(const void* gptr, uint32_t la) {
+    asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dword %0, off"
+                 :
+                 : "v"(gptr), "s"(la)
+                 : "memory", "m0");
+}
+
+// dma16 with a wave-uniform base (scalar registers) and a 32-bit per-lane
 // byte offset (no per-lane 64-bit address arithmetic).
 // NT: a streaming (nontemporal) load.
 template <bool NT = false>

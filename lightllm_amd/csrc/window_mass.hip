@@ -31,8 +31,9 @@ struct WindowArgs {
     int max_blocks, N, Hq, Hkv, D, bs, max_len;
     float scale_log2;
     int nblk;          // key blocks of a sequence, a wave's keys each (by the bound)
-    float* part;       // [rows * Hq][nblk] log2-sum-exp2 per key block
-    float* lse;        // [rows * Hq]
+    int64_t cols;      // rows x (Hq / Hkv) of the call
+    float* part;       // [nblk][Hkv][cols] log2-sum-exp2 per key block
+    float* lse;        // [Hkv][cols] (the generic kernels: [rows][Hq])
     float* mass;
     int64_t mass_bs, mass_hs;
 };
@@ -62,13 +63,28 @@ constexpr int wave_keys() { return 16 * key_tiles<T>(); }
 template <typename T, int D>
 constexpr int chunk_cols() { return D == 96 ? 512 / (int)sizeof(T) / 2 : 16384 / (D * (int)sizeof(T)); }
 
-// SUM false: part[column][wave] = the log2-sum-exp2 of each column over a wave's keys.
+// x and the value of the lane 16 (32) away, reduced: the four lanes of a column, which
+// lie in different rows of 16, by swaps of rows between two registers.
+template <class F>
+__device__ inline float over_rows(float x, F f) {
+    const uint32_t u = __float_as_uint(x);
+    const auto a = __builtin_amdgcn_permlane16_swap(u, u, false, false);
+    const uint32_t v = __float_as_uint(f(__uint_as_float(a[0]), __uint_as_float(a[1])));
+    const auto b = __builtin_amdgcn_permlane32_swap(v, v, false, false);
+    return f(__uint_as_float(b[0]), __uint_as_float(b[1]));
+}
+
+// SUM false: the log2-sum-exp2 of each column over a wave's keys, part[wave][kv head][column].
 // SUM true: the totals, from the columns' log2-sum-exp2.
 // Grid (nblk / W, Hkv, N), W waves.  The columns' rows go through LDS by direct loads,
 // a ring of three chunks that all waves read: read by each wave from the caches, they
 // took 6 TB/s from L2 and set the time (28/4/128 bf16, 2 x 30001 keys, 64 rows: 72 and
 // 100 us the two passes).  A row's 16-byte units are XOR-ed with the column (rotated by
-// it at head_dim 96), so that the 16 columns of an operand lie in different banks.
+// it at head_dim 96), so that the 16 columns of an operand lie in different banks.  The
+// second pass has its columns' log2-sum-exp2 in the ring as well, and the first stores a
+// chunk's results a chunk later, before it issues the loads of another one: vector
+// memory returns in order, so a load or store of its own behind those of the ring made
+// every step wait for the ring (53 us a pass).
 template <typename T, int D, int W, bool SUM>
 __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(D == 256 ? (sizeof(T) == 2 ? 2 : 1) : (D == 128 && sizeof(T) == 4 ? 3 : 4))))
 void window_kernel(WindowArgs a) {
@@ -76,9 +92,11 @@ void window_kernel(WindowArgs a) {
     constexpr int KT = key_tiles<T>();
     constexpr bool k16 = Elem<T>::kDtype != LLKV_DTYPE_F32;
     constexpr int NC = chunk_cols<T, D>(), CPR = D * (int)sizeof(T) / 16, R = 3;
-    constexpr int LPW = NC * CPR / (64 * W);   // loads of a lane per chunk
+    constexpr int NS = NC / 16, NK = (NC + 63) / 64;   // steps of 16 columns, column blocks of 64
+    constexpr int LPW = NC * CPR / (64 * W) + (SUM ? NK : 0);   // loads of a lane per chunk
     static_assert(NC % 16 == 0 && NC * CPR % (64 * W) == 0, "chunks are whole loads");
     __shared__ mu32x4 rows[R][NC * CPR];
+    __shared__ float lse_s[SUM ? R : 1][SUM ? 64 * NK : 1];
     const int n = blockIdx.z, kvh = blockIdx.y;
     const WindowSeq s = window_seq(a, n);
     if ((int)blockIdx.x * W * wave_keys<T>() >= s.L || s.P == 0) return;   // uniform over the work-group
@@ -89,22 +107,32 @@ void window_kernel(WindowArgs a) {
     const bool idle = k0 >= s.L;   // the wave has no key: it loads and waits only
     const int G = a.Hq / a.Hkv, cols = s.P * G, chunks = (cols + NC - 1) / NC;
     const int64_t row_elems = (int64_t)a.Hkv * D;
+    const float* const lse = a.lse + kvh * a.cols + (int64_t)s.q0 * G;
+    float* const part = a.part + ((int64_t)blk * a.Hkv + kvh) * a.cols + (int64_t)s.q0 * G;
 
     auto place = [](int col, int u) { return (CPR & (CPR - 1)) == 0 ? u ^ (col & (CPR - 1)) : (u + col) % CPR; };
     auto unit_at = [](int col, int pl) {
         return (CPR & (CPR - 1)) == 0 ? pl ^ (col & (CPR - 1)) : (pl + CPR * NC - col) % CPR;
     };
     const char* const qbase = reinterpret_cast<const char*>(a.q) + ((int64_t)s.q0 * a.Hq + kvh * G) * D * (int)sizeof(T);
-    uint32_t lds[LPW];
+    constexpr int RL = NC * CPR / (64 * W);   // of them rows
+    uint32_t lds[RL], lds_lse[NK];
 #pragma unroll
-    for (int i = 0; i < LPW; ++i) lds[i] = lds_addr(&rows[0][64 * (LPW * w + i)]);
+    for (int i = 0; i < RL; ++i) lds[i] = lds_addr(&rows[0][64 * (RL * w + i)]);
+#pragma unroll
+    for (int i = 0; i < NK; ++i) lds_lse[i] = lds_addr(&lse_s[0][SUM ? 64 * i : 0]);
     auto load_chunk = [&](int ch) {
 #pragma unroll
-        for (int i = 0; i < LPW; ++i) {
-            const int x = 64 * (LPW * w + i) + lane, r = x / CPR;
+        for (int i = 0; i < RL; ++i) {
+            const int x = 64 * (RL * w + i) + lane, r = x / CPR;
             const int col = min(ch * NC + r, cols - 1), node = col / G;   // (beyond the last: not used)
             const int64_t off = ((int64_t)node * a.Hq + (col - node * G)) * D * (int)sizeof(T) + unit_at(r, x % CPR) * 16;
             dma16(qbase + off, lds[i] + (uint32_t)(ch % R) * (NC * CPR * 16));
+        }
+        if constexpr (SUM) {   // every wave the same values: its own wait covers them
+#pragma unroll
+            for (int i = 0; i < NK; ++i)
+                dma4(lse + min(ch * NC + 64 * i + lane, cols - 1), lds_lse[i] + (uint32_t)(ch % R) * (64 * NK * 4));
         }
     };
     load_chunk(0);
@@ -120,48 +148,64 @@ void window_kernel(WindowArgs a) {
             Ops::template load_k<false>(reinterpret_cast<const T*>(a.k) + (int64_t)kvh * D + (phys * kPage + c) * row_elems,
                                         g, kr[kt]);
         }
+        // fp32 keys are scaled here, 16-bit scores in the exponent; a negative scale goes into
+        // the keys' signs, so that the largest score stays the largest when scaled.
+        if constexpr (k16) {
+            if (a.scale_log2 < 0.0f) {
+#pragma unroll
+                for (int kt = 0; kt < KT; ++kt)
+#pragma unroll
+                    for (int i = 0; i < Ops::NK; ++i) kr[kt][i] ^= 0x80008000u;
+            }
+        } else {
+#pragma unroll
+            for (int kt = 0; kt < KT; ++kt)
+#pragma unroll
+                for (int i = 0; i < Ops::NK; ++i) {
+                    kr[kt][i].x *= a.scale_log2;
+                    kr[kt][i].y *= a.scale_log2;
+                    kr[kt][i].z *= a.scale_log2;
+                    kr[kt][i].w *= a.scale_log2;
+                }
+        }
     }
     const bool whole = k0 + wave_keys<T>() <= s.hist;   // every row sees all of the wave's keys (uniform)
-    // 16-bit scores are scaled here, fp32 ones by their Q; under a negative scale they change
-    // sign first, so that the largest stays the largest.
     const float scale = k16 ? fabsf(a.scale_log2) : 1.0f;
-    const bool negative = k16 && a.scale_log2 < 0.0f;
 
     float sum[KT][4];
 #pragma unroll
     for (int kt = 0; kt < KT; ++kt)
 #pragma unroll
         for (int i = 0; i < 4; ++i) sum[kt][i] = 0.0f;
+    // The keys have arrived: left open, the compiler's waits for them stayed in the loop, where
+    // they meet the ring's loads.
+    __builtin_amdgcn_s_waitcnt(vmcnt_imm(0));
 
-    // Column 16 k + c is row `node` under head `head` of the group; the next 16 columns are
-    // 16 / G rows and 16 % G heads further.
-    const int step_node = 16 / G, step_head = 16 - step_node * G;
-    int node = c / G, head = c - node * G;
-    auto column_at = [&]() { return (int64_t)(s.q0 + node) * a.Hq + kvh * G + head; };
-    float next_lse = INFINITY;
-    if (SUM && c < cols) next_lse = a.lse[column_at()];
+    // First pass: the maximum and the sum of column 64 k + lane of a chunk.
+    float top_of[NK], sum_of[NK];
+    auto store_chunk = [&](int ch) {
+#pragma unroll
+        for (int k = 0; k < NK; ++k) {
+            const int x = 64 * k + lane, col = ch * NC + x;
+            if (x < NC && col < cols) part[col] = sum_of[k] == 0.0f ? -INFINITY : top_of[k] + fast_log2(sum_of[k]);
+        }
+    };
 
     for (int ch = 0; ch < chunks; ++ch) {
         if (ch + 1 < chunks) __builtin_amdgcn_s_waitcnt(vmcnt_imm(LPW));   // all but the next chunk's loads
         else __builtin_amdgcn_s_waitcnt(vmcnt_imm(0));
         lds_barrier();   // the chunk is there for all, and the one before it has been read
+        if constexpr (!SUM) {
+            if (ch > 0 && !idle) store_chunk(ch - 1);
+        }
         if (ch + 2 < chunks) load_chunk(ch + 2);
         if (idle) continue;
         const mu32x4* const here = rows[ch % R];
         const int stop = min(NC, cols - ch * NC);
-        for (int c0 = 0; c0 < stop; c0 += 16) {
-            const int col = ch * NC + c0 + c;
-            const int64_t at = column_at();
-            const int last = min(s.hist + node, s.L - 1) - k0 - 4 * g;   // the last key that the column sees
-            const float lse = next_lse;
-            node += step_node;
-            head += step_head;
-            node += head >= G ? 1 : 0;
-            head -= head >= G ? G : 0;
-            if constexpr (SUM) {   // a round ahead
-                next_lse = INFINITY;
-                if (col + 16 < cols) next_lse = a.lse[column_at()];
-            }
+#pragma unroll
+        for (int st = 0; st < NS; ++st) {
+            const int c0 = 16 * st;
+            if (c0 >= stop) break;   // (uniform)
             typename Ops::QReg q[Ops::NQ];
 #pragma unroll
             for (int i = 0; i < CPR / 4; ++i) {
@@ -170,51 +214,74 @@ void window_kernel(WindowArgs a) {
                     q[i] = x;
                 } else {
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) q[4 * i + e] = __uint_as_float(x[e]) * a.scale_log2;
+                    for (int e = 0; e < 4; ++e) q[4 * i + e] = __uint_as_float(x[e]);
                 }
             }
             mf32x4 x[KT];
+            if constexpr (k16) {   // k-step by k-step: four products that do not wait for each other
 #pragma unroll
-            for (int kt = 0; kt < KT; ++kt) x[kt] = Ops::scores(kr[kt], q, 1.0f);
-            if (negative) {
+                for (int ks = 0; ks < Ops::NK; ++ks) {
 #pragma unroll
-                for (int kt = 0; kt < KT; ++kt) x[kt] = -x[kt];
+                    for (int kt = 0; kt < KT; ++kt)
+                        x[kt] = Ops::mma(kr[kt][ks], q[ks], ks == 0 ? mf32x4{0.f, 0.f, 0.f, 0.f} : x[kt]);
+                }
+                __builtin_amdgcn_sched_group_barrier(0x100, Ops::NK, 0);
+                __builtin_amdgcn_sched_group_barrier(0x008, Ops::NK * KT, 0);
+            } else {
+#pragma unroll
+                for (int kt = 0; kt < KT; ++kt) x[kt] = Ops::scores(kr[kt], q, 1.0f);
             }
+            float f = scale;
             if (!whole) {
+                const int node = (ch * NC + c0 + c) / G;
+                const int last = min(s.hist + node, s.L - 1) - k0 - 4 * g;   // the last key that the column sees
 #pragma unroll
                 for (int kt = 0; kt < KT; ++kt)
 #pragma unroll
                     for (int i = 0; i < 4; ++i) x[kt][i] = 16 * kt + i <= last ? x[kt][i] * scale : -INFINITY;
+                f = 1.0f;   // (a masked score stays what it is under a scale of zero)
             }
-            const float f = whole ? scale : 1.0f;   // (a masked score stays what it is under a scale of zero)
             if constexpr (SUM) {
+                const float here_lse = lse_s[ch % R][c0 + c], l = c0 + c < stop ? here_lse : INFINITY;
 #pragma unroll
                 for (int kt = 0; kt < KT; ++kt)
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) sum[kt][i] += fast_exp2(fmaf(x[kt][i], f, -lse));
+                    for (int i = 0; i < 4; ++i) sum[kt][i] += fast_exp2(fmaf(x[kt][i], f, -l));
             } else {
-                float m = kNegBig, l = 0.0f;
+                // exp2 of the scores as they are: while a column's sum lies well within fp32's
+                // range, no maximum has to be taken off, which would not change its precision.
+                float top = 0.0f;
+                auto exps = [&]() {
+                    float l[4];
 #pragma unroll
-                for (int kt = 0; kt < KT; ++kt)
+                    for (int kt = 0; kt < KT; ++kt)
 #pragma unroll
-                    for (int i = 0; i < 4; i += 2) m = fmaxf(fmaxf(m, x[kt][i]), x[kt][i + 1]);
-                m *= f;
+                        for (int i = 0; i < 4; ++i) {
+                            const float e = fast_exp2(fmaf(x[kt][i], f, -top));
+                            l[i] = kt == 0 ? e : l[i] + e;
+                        }
+                    return over_rows((l[0] + l[1]) + (l[2] + l[3]), [](float u, float v) { return u + v; });
+                };
+                float all = exps();
+                if (__builtin_amdgcn_ballot_w64(!(all >= 0x1p-60f && all <= 0x1p100f)) != 0) {
+                    float m = kNegBig;
 #pragma unroll
-                for (int kt = 0; kt < KT; ++kt)
+                    for (int kt = 0; kt < KT; ++kt)
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) l += fast_exp2(fmaf(x[kt][i], f, -m));
-                // the four lanes of a column
-                float top = fmaxf(m, __shfl_xor(m, 16, 64));
-                top = fmaxf(top, __shfl_xor(top, 32, 64));
-                l *= fast_exp2(m - top);
-                l += __shfl_xor(l, 16, 64);
-                l += __shfl_xor(l, 32, 64);
-                if (g == 0 && col < cols) a.part[at * a.nblk + blk] = l == 0.0f ? -INFINITY : top + fast_log2(l);
+                        for (int i = 0; i < 4; i += 2) m = fmaxf(fmaxf(m, x[kt][i]), x[kt][i + 1]);
+                    top = over_rows(m * f, [](float u, float v) { return fmaxf(u, v); });
+                    all = exps();
+                }
+                const bool mine = g == (st & 3);
+                top_of[st / 4] = mine ? top : top_of[st / 4];
+                sum_of[st / 4] = mine ? all : sum_of[st / 4];
             }
         }
     }
-    if constexpr (SUM) {
-        if (idle) return;
+    if (idle) return;
+    if constexpr (!SUM) {
+        store_chunk(chunks - 1);
+    } else {
         float* mass = a.mass + n * a.mass_bs + kvh * a.mass_hs;
 #pragma unroll
         for (int kt = 0; kt < KT; ++kt)
@@ -228,24 +295,40 @@ void window_kernel(WindowArgs a) {
 }
 
 // Per column: the log2-sum-exp2 over its key blocks, +inf for a column that sees
-// no key (every weight is then zero).  Grid (rows of the longest window x Hq / 4, N), a wave per column.
+// no key (every weight is then zero).  Grid (groups of 16 columns, Hkv, N): 16 columns,
+// 16 threads each, with four blocks in flight.
 __global__ __launch_bounds__(256) void window_lse_kernel(WindowArgs a, int keys) {
-    const int n = blockIdx.y, lane = threadIdx.x & 63;
+    __shared__ float part_m[16][17], part_s[16][17];
+    const int n = blockIdx.z, kvh = blockIdx.y, c = threadIdx.x & 15, t = threadIdx.x >> 4;
     const WindowSeq s = window_seq(a, n);
-    const int nblk = (s.L + keys - 1) / keys;
-    for (int64_t r = blockIdx.x * 4 + (threadIdx.x >> 6); r < (int64_t)s.P * a.Hq; r += gridDim.x * 4) {
-        const int64_t at = (int64_t)s.q0 * a.Hq + r;
+    const int nblk = (s.L + keys - 1) / keys, cols = s.P * (a.Hq / a.Hkv);
+    const int64_t at = (int64_t)s.q0 * (a.Hq / a.Hkv), step = a.Hkv * a.cols;
+    for (int c0 = 16 * blockIdx.x; c0 < cols; c0 += 16 * gridDim.x) {   // (uniform)
+        const bool on = c0 + c < cols;
+        const float* part = a.part + kvh * a.cols + at + (on ? c0 + c : c0);
         float M = -INFINITY, S = 0.0f;
-        for (int j = lane; j < nblk; j += 64) {
-            const float x = a.part[at * a.nblk + j];
-            const float mb = fmaxf(M, x);
-            if (mb == -INFINITY) continue;
-            S = S * fast_exp2(M - mb) + fast_exp2(x - mb);
+        for (int j = t; j < nblk; j += 64) {
+            float x[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) x[i] = j + 16 * i < nblk ? part[(j + 16 * i) * step] : -INFINITY;
+            const float mb = fmaxf(fmaxf(M, fmaxf(x[0], x[1])), fmaxf(x[2], x[3]));
+            const float base = mb == -INFINITY ? 0.0f : mb;   // (a score that is no number stays one in the sum)
+            S *= fast_exp2(M - base);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) S += fast_exp2(x[i] - base);
             M = mb;
         }
-        const float top = wave_max(M);
-        S = wave_sum(top == -INFINITY ? 0.0f : S * fast_exp2(M - top));
-        if (lane == 0) a.lse[at] = S == 0.0f ? INFINITY : top + fast_log2(S);
+        __syncthreads();   // the columns before have been read
+        part_m[c][t] = M;
+        part_s[c][t] = S;
+        __syncthreads();
+        if (t == 0 && on) {
+            for (int i = 1; i < 16; ++i) M = fmaxf(M, part_m[c][i]);
+            const float base = M == -INFINITY ? 0.0f : M;
+            float sum = 0.0f;
+            for (int i = 0; i < 16; ++i) sum = fmaf(part_s[c][i], fast_exp2(part_m[c][i] - base), sum);
+            a.lse[kvh * a.cols + at + c0 + c] = sum == 0.0f ? INFINITY : M + fast_log2(sum);
+        }
     }
 }
 
@@ -283,13 +366,12 @@ __global__ __launch_bounds__(256) void window_lse_generic_kernel(WindowArgs a) {
         float M = -INFINITY, S = 0.0f;
         for (int j = lane; j < stop; j += 64) {
             const float x = dot(q, key_row<T>(a, n, kvh, j), a.D) * a.scale_log2;
-            const float mb = fmaxf(M, x);
-            if (mb == -INFINITY) continue;
-            S = S * fast_exp2(M - mb) + fast_exp2(x - mb);
+            const float mb = fmaxf(M, x), base = mb == -INFINITY ? 0.0f : mb;
+            S = S * fast_exp2(M - base) + fast_exp2(x - base);
             M = mb;
         }
         const float top = wave_max(M);
-        S = wave_sum(top == -INFINITY ? 0.0f : S * fast_exp2(M - top));
+        S = wave_sum(S * fast_exp2(M - (top == -INFINITY ? 0.0f : top)));
         if (lane == 0) a.lse[at] = S == 0.0f ? INFINITY : top + fast_log2(S);
     }
 }
@@ -317,9 +399,9 @@ int keys_of(int dtype) { return dtype == LLKV_DTYPE_F32 ? wave_keys<float>() : w
 template <typename T, int D, int W>
 void launch_waves(const WindowArgs& a, int max_q_len, hipStream_t st) {
     const dim3 grid((a.nblk + W - 1) / W, a.Hkv, a.N);
-    const int lse_wgs = (int)std::min<int64_t>(((int64_t)max_q_len * a.Hq + 3) / 4, 65535);
+    const int lse_wgs = (int)std::min<int64_t>(((int64_t)max_q_len * (a.Hq / a.Hkv) + 15) / 16, 65535);
     window_kernel<T, D, W, false><<<grid, 64 * W, 0, st>>>(a);
-    window_lse_kernel<<<dim3(lse_wgs, a.N), 256, 0, st>>>(a, wave_keys<T>());
+    window_lse_kernel<<<dim3(lse_wgs, a.Hkv, a.N), 256, 0, st>>>(a, wave_keys<T>());
     window_kernel<T, D, W, true><<<grid, 64 * W, 0, st>>>(a);
 }
 
@@ -410,6 +492,7 @@ extern "C" int llkv_paged_window_mass(float* mass, int64_t mass_seq_stride, int6
     a.max_len = max_seq_len;
     a.scale_log2 = scale * kLog2e;
     a.nblk = p.nblk;
+    a.cols = (int64_t)total_q * (num_q_heads / num_kv_heads);
     a.part = reinterpret_cast<float*>(workspace);
     a.lse = reinterpret_cast<float*>(reinterpret_cast<char*>(workspace) + p.lse);
     a.mass_bs = mass_seq_stride;
