@@ -427,16 +427,24 @@ struct ManyCols {
         const char* const kb = loads_v ? vp : kp;
         int tbl = 0;   // page ids of the wave's next 64 tiles, one per lane
         auto load_tile = [&](int j) {
-            if ((j & 63) == 0) tbl = bt[min((begin + (j + lane) * BN + part) / kPage, last_page)];
+            if ((j & 63) == 0) {
+                tbl = bt[min((begin + (j + lane) * BN + part) / kPage, last_page)];
+                // Waited for here: at its use, where the compiler cannot tell whether it is still
+                // on the way, the wait would stand in every tile and empty the ring.
+                __builtin_amdgcn_s_waitcnt(vmcnt_imm(0));
+            }
             const int phys = max(__builtin_amdgcn_readlane(tbl, j & 63), 0);
             const uint64_t base = (uint64_t)(uint32_t)phys * row_bytes * kPage;
             const uint32_t to = (uint32_t)(j % R) * kTileBytes;
+            if (sg.stream) {   // (uniform)
 #pragma unroll
-            for (int i = 0; i < BPW; ++i) {
-                if (sg.stream) {   // (uniform)
+                for (int i = 0; i < BPW; ++i) {
                     dma16_s<true>(kb + base, off[i], to_k[i] + to);
                     if constexpr (W == 4) dma16_s<true>(vp + base, off[i], to_v[i] + to);
-                } else {
+                }
+            } else {
+#pragma unroll
+                for (int i = 0; i < BPW; ++i) {
                     dma16_s(kb + base, off[i], to_k[i] + to);
                     if constexpr (W == 4) dma16_s(vp + base, off[i], to_v[i] + to);
                 }
