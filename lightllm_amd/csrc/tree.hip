@@ -378,6 +378,11 @@ struct ManyCols {
     static constexpr int kLoads = (W == 4 ? 2 : 1) * BPW;   // of a wave per tile
     static_assert((W == 4 || W == 8) && RPW * D * 2 % 1024 == 0 && kPage % RPW == 0, "tile parts");
     static constexpr int kWavesPerEU = 2;
+    // Eight waves, two per SIMD: the second four run half a tile behind (kPair), so that the
+    // exponentials of the one meet the products of the other (32/8/128 fp16, 32 x 2816 keys,
+    // 64 nodes: 120 us all at once, 110 so).
+    static constexpr bool kPair = W == 8 && !MASS;
+    static constexpr int kAhead = kPair ? R - 2 : R - 1;   // tiles loaded ahead (V of tile j - 1 is still read)
     static constexpr bool kMass = MASS, kTeams = !MASS, kStreams = true;
     static constexpr uint32_t kOnes = Elem<T>::kDtype == LLKV_DTYPE_F16 ? 0x3C003C00u : 0x3F803F80u;
     static constexpr bool kF16 = Elem<T>::kDtype == LLKV_DTYPE_F16;
@@ -388,14 +393,23 @@ struct ManyCols {
         int odd;
     };
 
-    // Place of chunk ch of row r, and the chunk at a place: XOR with row bits 0, 1, 3, 4 (the
-    // rows that an operand read takes together differ there), or a rotation by them where a
-    // row's chunks are no power of two.
+    // Place of chunk ch of row r, and the chunk at a place: XOR with row bits, or a rotation by
+    // them where a row's chunks are no power of two.  K: bits 0, 1, 3, 4 (the 16 rows that an
+    // operand read takes together differ there).  V: 8 rows of 32 lanes, which read pairs of
+    // chunks: bits 0, 1, 3 (at head_dim 64, where two rows share the banks, 1 and 3) above the
+    // pair (with K's bits, two rows' pairs met in the same banks).
     static constexpr bool kXor = (CPR & (CPR - 1)) == 0;
-    __device__ static int bits(int r) { return (r & 3) | ((r >> 1) & 0xC); }
-    __device__ static int place(int r, int ch) { return kXor ? ch ^ (bits(r) & (CPR - 1)) : (ch + bits(r)) % CPR; }
-    __device__ static int chunk(int r, int pl) { return kXor ? pl ^ (bits(r) & (CPR - 1)) : (pl + 16 * CPR - bits(r)) % CPR; }
-    __device__ static int at(int row, int d) { return row * D + (place(row, d >> 3) << 3 | (d & 7)); }
+    template <bool V>
+    __device__ static int bits(int r) {
+        if (kXor && V) return CPR == 8 ? (r & 2) | ((r & 8) >> 1) : ((r & 3) << 1) | (r & 8);
+        return ((r & 3) | ((r >> 1) & 0xC)) & (kXor ? CPR - 1 : ~0);
+    }
+    template <bool V>
+    __device__ static int place(int r, int ch) { return kXor ? ch ^ bits<V>(r) : (ch + bits<V>(r)) % CPR; }
+    template <bool V>
+    __device__ static int chunk(int r, int pl) { return kXor ? pl ^ bits<V>(r) : (pl + 16 * CPR - bits<V>(r)) % CPR; }
+    template <bool V>
+    __device__ static int at(int row, int d) { return row * D + (place<V>(row, d >> 3) << 3 | (d & 7)); }
 
     __device__ static void run(const TreeArgs& a, Smem& sm, const TreeSeg& sg) {
         const int tid = threadIdx.x, lane = tid & 63;
@@ -416,11 +430,13 @@ struct ManyCols {
         constexpr uint32_t kTileBytes = BN * D * 2;
         const int part = RPW * (w & 3);   // first row
         const bool loads_v = W == 8 && w >= 4;
-        uint32_t off[BPW], to_k[BPW], to_v[BPW];
+        uint32_t off[BPW], off_v[BPW], to_k[BPW], to_v[BPW];   // (off: V's in the waves that load only V)
 #pragma unroll
         for (int i = 0; i < BPW; ++i) {
             const int u = 64 * i + lane, r = part + u / CPR;
-            off[i] = (uint32_t)(r % kPage) * row_bytes + (uint32_t)chunk(r, u % CPR) * 16u;
+            const uint32_t row = (uint32_t)(r % kPage) * row_bytes;
+            off_v[i] = row + (uint32_t)chunk<true>(r, u % CPR) * 16u;
+            off[i] = loads_v ? off_v[i] : row + (uint32_t)chunk<false>(r, u % CPR) * 16u;
             to_k[i] = lds_addr((loads_v ? sm.v[0] : sm.k[0]) + part * D + 512 * i);
             to_v[i] = lds_addr(sm.v[0] + part * D + 512 * i);
         }
@@ -440,27 +456,23 @@ struct ManyCols {
 #pragma unroll
                 for (int i = 0; i < BPW; ++i) {
                     dma16_s<true>(kb + base, off[i], to_k[i] + to);
-                    if constexpr (W == 4) dma16_s<true>(vp + base, off[i], to_v[i] + to);
+                    if constexpr (W == 4) dma16_s<true>(vp + base, off_v[i], to_v[i] + to);
                 }
             } else {
 #pragma unroll
                 for (int i = 0; i < BPW; ++i) {
                     dma16_s(kb + base, off[i], to_k[i] + to);
-                    if constexpr (W == 4) dma16_s(vp + base, off[i], to_v[i] + to);
+                    if constexpr (W == 4) dma16_s(vp + base, off_v[i], to_v[i] + to);
                 }
             }
         };
-#pragma unroll
-        for (int j = 0; j < R - 1; ++j)
-            if (j < tiles) load_tile(j);
-
         // Where the lane's operands lie in a tile (halves): K row 8 (c / 4) + c % 4 for each
         // k-step, V row 8 g + c / 4 for each output tile.
         int koff[KS], voff[DT];
 #pragma unroll
-        for (int ks = 0; ks < KS; ++ks) koff[ks] = at(8 * (c >> 2) + (c & 3), ks * 32 + g * 8);
+        for (int ks = 0; ks < KS; ++ks) koff[ks] = at<false>(8 * (c >> 2) + (c & 3), ks * 32 + g * 8);
 #pragma unroll
-        for (int dt = 0; dt < DT; ++dt) voff[dt] = at(8 * g + (c >> 2), dt * 16 + 4 * (c & 3));
+        for (int dt = 0; dt < DT; ++dt) voff[dt] = at<true>(8 * g + (c >> 2), dt * 16 + 4 * (c & 3));
 
         // Columns; a negative scale goes into Q's signs, so that the largest score stays the
         // largest when scaled.
@@ -491,48 +503,22 @@ struct ManyCols {
             m[nt] = kNegBig;
             l[nt] = 0.0f;
         }
+        __builtin_amdgcn_sched_barrier(0);   // Q before the tiles (loads return in order)
+#pragma unroll
+        for (int j = 0; j < kAhead; ++j)
+            if (j < tiles) load_tile(j);
         const mu32x4 ones = {kOnes, kOnes, kOnes, kOnes};
         bool odd = false;
         const bool idle = sg.c0 + w * NCW * 16 >= sg.cols;   // the wave has no column: it loads and waits only
 
-        for (int j = 0; j < tiles; ++j) {
-            // This wave's part of tile j is in LDS: all loads but those of the tiles after it.
-            const int after = tiles - 1 - j;
-            constexpr int kAll = vmcnt_imm(kLoads * (R - 2)), kLess = vmcnt_imm(R > 2 ? kLoads * (R - 3) : 0);
-            if (after >= R - 2) __builtin_amdgcn_s_waitcnt(kAll);
-            else if (after == R - 3) __builtin_amdgcn_s_waitcnt(kLess);
-            else __builtin_amdgcn_s_waitcnt(vmcnt_imm(0));
-            lds_barrier();   // everyone's; and the buffer of tile j - 1 has been read
-            if (j + R - 1 < tiles) load_tile(j + R - 1);
-            uint16_t* const kt_lds = sm.k[j % R];
-            uint16_t* const vt_lds = sm.v[j % R];
-            // V^T operand of output dims 16 dt .. + 15 and the 32-key half ss.
-            auto v_operand = [&](int dt, int ss) {
-                typedef short s16x4 __attribute__((ext_vector_type(4)));
-                const uint16_t* at0 = vt_lds + voff[dt] + 32 * ss * D;
-                const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)at0);
-                const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(at0 + 4 * D));
-                const mu32x2 l2 = __builtin_bit_cast(mu32x2, lo), h2 = __builtin_bit_cast(mu32x2, hi);
-                return mu32x4{l2.x, l2.y, h2.x, h2.y};
-            };
+        mu32x4 p[SS][NCW];   // the weights of a tile, packed
+        // S^T = K Q^T of tile j, masked, the running maximum, and the weights.
+        auto score = [&](int j, bool whole) {
+            const uint16_t* const kt_lds = sm.k[j % R];
             const int key0 = begin + j * BN;
-            const bool whole = key0 + BN <= min(hist, L);   // uniform
-            if (!whole) {
-                // V beyond the last key may hold anything: zero.  Values in the tree that are not
-                // finite: the segment is computed again.
-                for (int i = tid; i < BN * CPR; i += kThreads) {
-                    const int r = i / CPR;
-                    mu32x4& x = *reinterpret_cast<mu32x4*>(vt_lds + i * 8);
-                    if (key0 + r >= L) x = mu32x4{0u, 0u, 0u, 0u};
-                    else if (!MASS && key0 + r >= hist)
-                        odd |= !(finite_bits(x.x, kF16) && finite_bits(x.y, kF16) && finite_bits(x.z, kF16) && finite_bits(x.w, kF16));
-                }
-                lds_barrier();
-            }
-            if (idle) continue;   // (uniform over the wave)
             __builtin_amdgcn_sched_barrier(0);   // the next tile's loads are issued first
             if constexpr (D >= 128) __builtin_amdgcn_s_setprio(1);
-            // S^T = K Q^T, the K operands of k-step ks + 1 read behind the products of ks
+            // the K operands of k-step ks + 1 read behind the products of ks
             mf32x4 s[KT][NCW];
             auto k_operand = [&](int kt, int ks) {
                 return *reinterpret_cast<const mu32x4*>(kt_lds + koff[ks] + (32 * (kt >> 1) + 4 * (kt & 1)) * D);
@@ -605,58 +591,84 @@ struct ManyCols {
                     for (int dt = 0; dt < DT; ++dt) o[nt][dt] *= corr;
                 }
             }
-            // P in the pool's type (half a step of each weight, as the prefill), its row sums by
-            // the same rounded weights; O^T += V^T P^T.  The exponentials of the second 32 keys
-            // are spread between the products of the first.
-            auto weight = [&](int ss, int nt, int i) {
-                const float p = fast_exp2(fmaf(s[2 * ss + (i >> 2)][nt][i & 3], scale, -m[nt]));
-                if constexpr (MASS) l[nt] += p;
-                return p;
-            };
-            auto pack = [&](const float* e) {
-                return mu32x4{pack_pair<T>(e[0], e[1]), pack_pair<T>(e[2], e[3]), pack_pair<T>(e[4], e[5]), pack_pair<T>(e[6], e[7])};
-            };
-            mu32x4 p[NCW], va[DT];
-            float e1[NCW][8];
+            // P in the pool's type (half a step of each weight, as the prefill)
 #pragma unroll
-            for (int nt = 0; nt < NCW; ++nt) {
-                float e[8];
+            for (int ss = 0; ss < SS; ++ss)
 #pragma unroll
-                for (int i = 0; i < 8; ++i) e[i] = weight(0, nt, i);
-                p[nt] = pack(e);
-            }
+                for (int nt = 0; nt < NCW; ++nt) {
+                    float e[8];
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) {
+                        e[i] = fast_exp2(fmaf(s[2 * ss + (i >> 2)][nt][i & 3], scale, -m[nt]));
+                        if constexpr (MASS) l[nt] += e[i];
+                    }
+                    p[ss][nt] = mu32x4{pack_pair<T>(e[0], e[1]), pack_pair<T>(e[2], e[3]), pack_pair<T>(e[4], e[5]),
+                                       pack_pair<T>(e[6], e[7])};
+                }
+        };
+        // O^T += V^T P^T of tile j, and the row sums by the same rounded weights.
+        auto product = [&](int j) {
+            const uint16_t* const vt_lds = sm.v[j % R];
+            // V^T operand of output dims 16 dt .. + 15 and the 32-key half ss.
+            auto v_operand = [&](int dt, int ss) {
+                typedef short s16x4 __attribute__((ext_vector_type(4)));
+                const uint16_t* at0 = vt_lds + voff[dt] + 32 * ss * D;
+                const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)at0);
+                const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(at0 + 4 * D));
+                const mu32x2 l2 = __builtin_bit_cast(mu32x2, lo), h2 = __builtin_bit_cast(mu32x2, hi);
+                return mu32x4{l2.x, l2.y, h2.x, h2.y};
+            };
+            mu32x4 va[DT];
 #pragma unroll
             for (int dt = 0; dt < DT; ++dt) va[dt] = v_operand(dt, 0);
-            constexpr int kMf = (DT + 1) * NCW;   // products per half
-            if constexpr (SS == 2) __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-            for (int k = 0; k < kMf; ++k) {
-                const int dt = k / NCW, nt = k % NCW;
-                if (dt < DT) {
-                    o[nt][dt] = mma32<T>(va[dt], p[nt], o[nt][dt]);
-                    if (SS == 2 && nt == NCW - 1) va[dt] = v_operand(dt, 1);
-                } else if constexpr (!MASS) {
-                    osum[nt] = mma32<T>(ones, p[nt], osum[nt]);
+            for (int ss = 0; ss < SS; ++ss) {
+#pragma unroll
+                for (int dt = 0; dt < DT; ++dt) {
+#pragma unroll
+                    for (int nt = 0; nt < NCW; ++nt) o[nt][dt] = mma32<T>(va[dt], p[ss][nt], o[nt][dt]);
+                    if (ss + 1 < SS) {
+                        va[dt] = v_operand(dt, ss + 1);
+                        __builtin_amdgcn_sched_barrier(0);
+                    }
                 }
-                if constexpr (SS == 2) {
-#pragma unroll
-                    for (int e = k * 8 * NCW / kMf; e < (k + 1) * 8 * NCW / kMf; ++e) e1[e >> 3][e & 7] = weight(1, e >> 3, e & 7);
-                    __builtin_amdgcn_sched_barrier(0);
-                }
-            }
-            if constexpr (SS == 2) {
-#pragma unroll
-                for (int nt = 0; nt < NCW; ++nt) p[nt] = pack(e1[nt]);
-#pragma unroll
-                for (int dt = 0; dt < DT; ++dt)
-#pragma unroll
-                    for (int nt = 0; nt < NCW; ++nt) o[nt][dt] = mma32<T>(va[dt], p[nt], o[nt][dt]);
                 if constexpr (!MASS) {
 #pragma unroll
-                    for (int nt = 0; nt < NCW; ++nt) osum[nt] = mma32<T>(ones, p[nt], osum[nt]);
+                    for (int nt = 0; nt < NCW; ++nt) osum[nt] = mma32<T>(ones, p[ss][nt], osum[nt]);
                 }
             }
+        };
+        const bool behind = kPair && w >= 4;   // (uniform over the wave)
+
+        for (int j = 0; j < tiles; ++j) {
+            // This wave's part of tile j is in LDS: all loads but those of the tiles after it.
+            const int after = tiles - 1 - j;
+            constexpr int kAll = vmcnt_imm(kLoads * (kAhead - 1)), kLess = vmcnt_imm(kAhead > 1 ? kLoads * (kAhead - 2) : 0);
+            if (after >= kAhead - 1) __builtin_amdgcn_s_waitcnt(kAll);
+            else if (after == kAhead - 2) __builtin_amdgcn_s_waitcnt(kLess);
+            else __builtin_amdgcn_s_waitcnt(vmcnt_imm(0));
+            lds_barrier();   // everyone's; and the buffer of the tile loaded next has been read
+            if (j + kAhead < tiles) load_tile(j + kAhead);
+            const int key0 = begin + j * BN;
+            const bool whole = key0 + BN <= min(hist, L);   // uniform
+            if (!whole) {
+                // V beyond the last key may hold anything: zero.  Values in the tree that are not
+                // finite: the segment is computed again.
+                for (int i = tid; i < BN * CPR; i += kThreads) {
+                    const int r = i / CPR;
+                    mu32x4& x = *reinterpret_cast<mu32x4*>(sm.v[j % R] + i * 8);
+                    if (key0 + r >= L) x = mu32x4{0u, 0u, 0u, 0u};
+                    else if (!MASS && key0 + r >= hist)
+                        odd |= !(finite_bits(x.x, kF16) && finite_bits(x.y, kF16) && finite_bits(x.z, kF16) && finite_bits(x.w, kF16));
+                }
+                lds_barrier();
+            }
+            if (idle) continue;   // (uniform over the wave)
+            if (behind && j > 0) product(j - 1);
+            score(j, whole);
+            if (!behind) product(j);
         }
+        if (behind && !idle && tiles > 0) product(tiles - 1);
         if constexpr (MASS) {
             lds_barrier();   // the last tile has been read: the next segment loads into the ring
         } else if (odd_segment(sm.odd, odd)) {
