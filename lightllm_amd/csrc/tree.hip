@@ -1195,21 +1195,20 @@ TreeChoice choose_f32(int64_t cols, int64_t tiles, bool mass) {
 
 // 16-bit pools.  From 129 columns on, units of 256 where there are tiles for 16 a
 // compute unit and most of the last unit is columns (32/8/128, 16 x 4500 keys, 64
-// nodes: 95 us, 113 by units of 64; 1000 tiles: 53 us and 39), else units of 64.  Up to
-// 128 one unit of 128 with eight waves and four tiles in flight (32 columns of 128 dims
-// 56 us, 59 by units of 64 on four waves); at head_dim 256 from 65 columns on (61 x
-// 1100 keys, 16 columns: 93 us, 84 by units of 64).
+// nodes: 102 us, 117 by units of 64; 16 x 500 keys: 41 us and 27), else units of 64.  Up
+// to 128, and at head_dim 256, one unit of 128 with eight waves and four tiles in the ring
+// (16 x 4500 keys, 8 nodes: 61 us, 64 by units of 64 on four waves; 16/8/256, 61 x 1100
+// keys, 8 nodes: 102 us and 110).
 template <typename T, int D>
 TreeChoice choose_16(int64_t cols, int64_t tiles, bool mass) {
     if (mass) return choice<ManyCols<T, D, 1, 8, 4, true>>();
     if constexpr (D <= 128) {
-        if (cols <= 128) return choice<ManyCols<T, D, 1, 8, 4>>();
-        if (tiles >= 16 * device_cus() && (cols - 1) % 256 >= 192) return choice<ManyCols<T, D, 2, 8, 4>>();
-        return choice<ManyCols<T, D, 1, 4, 2>>();
-    } else {
-        if (cols <= 64) return choice<ManyCols<T, D, 1, 4, 2>>();
-        return choice<ManyCols<T, D, 1, 8, 4>>();
+        if (cols > 128) {
+            if (tiles >= 16 * device_cus() && (cols - 1) % 256 >= 192) return choice<ManyCols<T, D, 2, 8, 4>>();
+            return choice<ManyCols<T, D, 1, 4, 2>>();
+        }
     }
+    return choice<ManyCols<T, D, 1, 8, 4>>();
 }
 
 template <typename T, int D>
