@@ -845,13 +845,14 @@ __device__ inline void join_columns(const TreeArgs& a, JoinSmem& sm, int cols, i
             float mb = M;
 #pragma unroll
             for (int b = 0; b < kBatch; ++b) mb = fmaxf(mb, lv[b]);
-            if (mb == -INFINITY) continue;   // no key seen so far
-            const float sc = fast_exp2(M - mb);
+            // (no key seen so far: weights of zero; a part that is no number stays one)
+            const float base = mb == -INFINITY ? 0.0f : mb;
+            const float sc = fast_exp2(M - base);
             sum *= sc;
             o *= sc;
 #pragma unroll
             for (int b = 0; b < kBatch; ++b) {
-                const float f = fast_exp2(lv[b] - mb);
+                const float f = fast_exp2(lv[b] - base);
                 sum += f;
                 o += f * pv[b];
             }
@@ -868,15 +869,14 @@ __device__ inline void join_columns(const TreeArgs& a, JoinSmem& sm, int cols, i
         if (sub == 0) {
             float top = M;
             for (int i = 1; i < sp; ++i) top = fmaxf(top, sm.ml[r + i][0]);
-            if (top > -INFINITY) {
-                float f = fast_exp2(M - top);
-                sum *= f;
-                o *= f;
-                for (int i = 1; i < sp; ++i) {
-                    f = fast_exp2(sm.ml[r + i][0] - top);
-                    sum = fmaf(f, sm.ml[r + i][1], sum);
-                    o += f * sm.o[threadIdx.x + i * LR];
-                }
+            const float base = top == -INFINITY ? 0.0f : top;
+            float f = fast_exp2(M - base);
+            sum *= f;
+            o *= f;
+            for (int i = 1; i < sp; ++i) {
+                f = fast_exp2(sm.ml[r + i][0] - base);
+                sum = fmaf(f, sm.ml[r + i][1], sum);
+                o += f * sm.o[threadIdx.x + i * LR];
             }
         }
         __syncthreads();
@@ -995,13 +995,12 @@ __global__ __launch_bounds__(256) void mass_join_kernel(TreeArgs a, int cols) {
             float M = -INFINITY, sum = 0.0f;
             for (int j = lane; j < parts; j += 64) {
                 const float y = a.part_lse[(int64_t)part_slot(w, u.slot, 1, j) * cols + c];
-                const float mb = fmaxf(M, y);
-                if (mb == -INFINITY) continue;
-                sum = sum * fast_exp2(M - mb) + fast_exp2(y - mb);
+                const float mb = fmaxf(M, y), base = mb == -INFINITY ? 0.0f : mb;
+                sum = sum * fast_exp2(M - base) + fast_exp2(y - base);
                 M = mb;
             }
             const float top = wave_max(M);
-            sum = wave_sum(top == -INFINITY ? 0.0f : sum * fast_exp2(M - top));
+            sum = wave_sum(sum * fast_exp2(M - (top == -INFINITY ? 0.0f : top)));
             v = top + fast_log2(sum);
         }
         if (lane == 0) lse[c] = v == -INFINITY ? INFINITY : v;   // no finite score: no weight

@@ -395,6 +395,24 @@ def test_one_long_context(dtype, d):
     check_mass(win[0].cpu(), torch.zeros(1, n), w.sum(1), n, err + p * hq * E, "window")
 
 
+@pytest.mark.parametrize("n", [40, 9000])
+@pytest.mark.parametrize("dtype", DTYPES, ids=IDS)
+def test_queries_that_are_no_numbers(dtype, n):
+    """Rows of NaN give NaN, and no other row does, whether or not their keys are cut into parts."""
+    c = Big([n], 1, 64, dtype)
+    q = torch.randn(3, 2, 64, generator=torch.Generator().manual_seed(2)).to(dtype).to(DEV)
+    q[1] = float("nan")
+    words = pack_mask([ancestors([-1, -1, -1])], 1).to(DEV)
+    got = kc.paged_tree_attention(q, c.kp, c.vp, c.dev_table, i32([0, 3]), c.dev_lens, words, 3, n)
+    assert torch.isnan(got[1]).all() and torch.isfinite(got[[0, 2]]).all()
+    mass = torch.zeros(1, 1, n, device=DEV)
+    out = kc.paged_decode_mass(q[1:2], c.kp, c.vp, c.dev_table, c.dev_lens, n, mass)
+    assert torch.isnan(out).all() and torch.isnan(mass).all()
+    win = torch.zeros(1, 1, n, device=DEV)
+    kc.paged_window_mass(q[1:2], c.kp, c.dev_table, i32([0, 1]), c.dev_lens, 1, n, win)
+    assert torch.isnan(win).all()
+
+
 def test_pools_of_more_than_2_to_32_elements():
     """Rows whose offsets do not fit 32 bits."""
     hq, hkv, d, lens, nodes = 8, 8, 128, [700, 90], [9, 4]
